@@ -199,6 +199,9 @@ enum molot_kv_dtype {
   MOLOT_KV_BF16 = 1, /* half the bytes; the reference specifies but does not
                         implement it: results match the reference run on the
                         bf16-rounded cache */
+  MOLOT_KV_F8B = 3,  /* page pools only (molot_pager_create_ex, molot_f8b_*):
+                       FP8 E4M3 codes with one scale per 16 slots and head;
+                       a KV handle and a paged plan refuse it */
   MOLOT_KV_Q8 = 2 /* ~0.28x the bytes (the Q8 KV of the reference's design,
                      DESIGN.md:48,87-88, deferred at exp/README.md:36-39): a
                      row is hd int8 codes then hd/32 FP32 scales, padded to
@@ -409,8 +412,118 @@ int molot_pager_free_pages(const molot_pager* p);
 /* Host block table [B][max_pages_per_seq] (unused entries 0) and lengths of
  * the batch `seqs`, ready for molot_paged_plan_build / molot_paged_decode. */
 int molot_pager_tables(molot_pager* p, const int* seqs, int B, int* block_table, int* seq_lens);
-/* Device K/V pools of one layer. */
+/* Device K/V pools of one layer (MOLOT_KV_F8B: the code pools). */
 int molot_pager_layer_pools(molot_pager* p, int layer, float** k_pool, float** v_pool);
+/* MOLOT_KV_F8B pools only: a layer's scales ([num_pages][nkv][page_size/16]
+ * each) and weight counters ([num_pages][nkv][page_size], zero at first).
+ * Any of the pointers may be NULL. */
+int molot_pager_layer_blocks(molot_pager* p, int layer, float** k_scale, float** v_scale,
+                             float** weight);
+
+/* ------------------------------------------------------------------------
+ * 8-bit block-scaled paged cache (no counterpart in the reference, which
+ * designs an 8-bit cache with per-row scales; see MOLOT_KV_Q8).
+ *
+ * Pools: K and V each [num_pages][nkv][page_size][d] FP8 E4M3 codes,
+ * page_size a multiple of 16, and one FP32 scale, a power of two, per block
+ * of 16 slots and head, [num_pages][nkv][page_size/16]: a slot's value is
+ * code * scale.  A block's scale is 2^e with the smallest e in [-64, 120]
+ * for which its largest finite magnitude is at most 448 * 2^e; codes are
+ * rounded to nearest even, infinities saturate, NaN stays NaN.
+ * Optionally, [num_pages][nkv][page_size] FP32 counters of the attention
+ * weight each slot has received.
+ *
+ * Rows, queries and outputs are FP32, BF16 or FP16 (molot_act_dtype); sums
+ * and softmax statistics are FP32.  Rows and queries are 16-byte aligned,
+ * with a stride in elements between tokens (heads are d elements apart), so
+ * they can be parts of one projection's output.
+ *
+ * A plan fixes a batch for one step (all layers): build it once per step,
+ * then call write / decode per layer, all on one stream.
+ * ---------------------------------------------------------------------- */
+enum molot_act_dtype { MOLOT_ACT_F32 = 0, MOLOT_ACT_BF16 = 1, MOLOT_ACT_F16 = 2 };
+
+/* One layer's device pointers and the batch's block table [B][max_pages]. */
+typedef struct molot_f8b_layer {
+  void* k;              /* code pools, 16-byte aligned */
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  float* weight;        /* counters; NULL where no call needs them */
+  const int* block_table;
+  int max_pages, page_size;
+} molot_f8b_layer;
+
+typedef struct molot_f8b_plan molot_f8b_plan;
+
+int molot_f8b_plan_create(molot_f8b_plan** out);
+void molot_f8b_plan_destroy(molot_f8b_plan* plan);
+/* Host arrays of B: seq_lens (slots with the step's new rows), new_lens (how
+ * many of them are new: the rows molot_f8b_write brings; NULL: 1 each),
+ * starts (first visible slot, e.g. of the newest of several documents in a
+ * sequence; NULL: 0) and prefix.  With pos = seq_lens - 1 a decode sees slot t
+ * when t >= start and (window <= 0, or pos - t < window, or
+ * t < start + prefix).  d 64, 128 or 256; nq / nkv at most 64. */
+int molot_f8b_plan_build(molot_f8b_plan* plan, int B, int nq, int nkv, int d, const int* seq_lens,
+                         const int* new_lens, const int* starts, const int* prefix, int window,
+                         void* stream);
+/* Quantizes the step's new rows, k and v [sum of new_lens][nkv][d], into
+ * slots [seq_len - new_len, seq_len) of their sequences; their counters
+ * become 0 where the layer has any.  A block that holds older rows keeps at
+ * least its scale; when that has to grow, the older codes are rounded to it. */
+int molot_f8b_write(molot_f8b_plan* plan, const molot_f8b_layer* layer, const void* k,
+                    const void* v, int act_dtype, long long k_stride, long long v_stride,
+                    void* stream);
+/* Attention of one query per sequence, q [B][nq][d] -> o [B][nq][d]
+ * (contiguous) over the visible slots: s = scale * q.k, then softcap *
+ * tanh(s / softcap) when softcap > 0, then - slopes[head] * (pos - t) when
+ * slopes (device, [nq]) is given, softmax, times V.  A sequence that sees
+ * nothing gives zeros.  lse (device, [B][nq], may be NULL) receives the
+ * natural logarithm of the softmax's sum (-inf when nothing is seen).
+ * With weight_out (a counter pool, layer->weight itself allowed), each slot
+ * of each sequence gets layer->weight plus its softmax weights summed over
+ * the kv head's queries; the first such call of a larger batch allocates
+ * scratch. */
+int molot_f8b_decode(molot_f8b_plan* plan, const molot_f8b_layer* layer, const void* q, void* o,
+                     float* lse, int act_dtype, long long q_stride, float scale, float softcap,
+                     const float* slopes, float* weight_out, void* stream);
+/* Per sequence and kv head, keeps `budget` of the plan's seq_len slots: the
+ * newest `recent`, and of the others those with the largest counters (equal
+ * ones: the lowest slot first; NaN last).  Their rows move, in order, to
+ * slots [0, budget) of dst (the same shape of pools; pages of its own block
+ * table, none of them the source's), quantized anew in their new blocks,
+ * their counters with them.  kept (device, [B][nkv][budget]) receives the
+ * source slots, ascending.  A sequence of at most `budget` slots moves
+ * whole, -1 in the rest of its kept row.  After it the new sequences have
+ * min(seq_len, budget) slots and the source's pages can be freed.  Heads keep
+ * different slots, so a window or distance bias counts kept slots after it. */
+int molot_f8b_evict(molot_f8b_plan* plan, const molot_f8b_layer* src, const molot_f8b_layer* dst,
+                    int budget, int recent, int* kept, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Prefill attention over packed documents (no counterpart in the reference;
+ * its prefill attention, gemm.h:409-446, takes one sequence and a window).
+ * Document i has q_lens[i] query rows, its last ones, and k_lens[i] key rows
+ * (NULL: q_lens); rows of all documents follow one another.  Query row m sits
+ * at position k_len - q_len + m and sees key t of its document when t <= pos
+ * and (window <= 0 or pos - t < window), or t < prefix[i] (NULL: 0).
+ * ---------------------------------------------------------------------- */
+typedef struct molot_packed_plan molot_packed_plan;
+
+int molot_packed_plan_create(molot_packed_plan** out);
+void molot_packed_plan_destroy(molot_packed_plan* plan);
+/* Host arrays of ndocs.  d 64, 128 or 256. */
+int molot_packed_plan_build(molot_packed_plan* plan, int ndocs, int nq, int nkv, int d,
+                            const int* q_lens, const int* k_lens, const int* prefix, int window,
+                            void* stream);
+/* q [rows][nq][d], k and v [keys][nkv][d] (strides in elements between rows,
+ * 16-byte aligned), o [rows][nq][d] contiguous, all MOLOT_ACT_BF16 or all
+ * MOLOT_ACT_F16.  Scores as in molot_f8b_decode, with the distance
+ * |pos - t|; a row that sees nothing gives zeros; lse [rows][nq] or NULL. */
+int molot_packed_attend(molot_packed_plan* plan, const void* q, const void* k, const void* v,
+                        void* o, float* lse, int act_dtype, long long q_stride,
+                        long long k_stride, long long v_stride, float scale, float softcap,
+                        const float* slopes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -14,6 +14,9 @@ and error behaviour mirror the reference's functions
 * ``KVCache`` (forward.h's per-layer KVC, HBM-resident) with
   ``append_rope`` / ``decode``;
 * ``PagedPlan`` for batched decode over 16-token pages;
+* ``F8Plan`` / ``F8Layer`` for the 8-bit block-scaled paged cache: writing
+  rows, decode attention, eviction by accumulated attention weight;
+* ``PackedPlan`` for prefill attention over packed documents;
 * ``Comm``, the peer-gather group of kv-head-sharded decode over several
   GPUs (``PagedPlan.decode_gather``).
 
@@ -45,7 +48,12 @@ ERR_NO_DEVICE = -8
 KV_F32 = 0   # molot_kv_dtype: the reference's FP32 cache
 KV_BF16 = 1  # BF16 storage (rounded on entry), FP32 math
 KV_Q8 = 2    # int8 codes + per-32 FP32 scales per row, FP32 math
+KV_F8B = 3  # page pools only: FP8 E4M3 codes, one scale per 16 slots and head
 _KV_DTYPES = {"f32": KV_F32, "bf16": KV_BF16, "q8": KV_Q8}
+
+
+_POOL_DTYPES = dict(_KV_DTYPES, f8b=KV_F8B)
+_ACT_DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}  # molot_act_dtype
 
 
 def q8_row_bytes(hd: int) -> int:
@@ -155,6 +163,25 @@ _decl("molot_comm_check", [_p, _p])
 _decl("molot_comm_destroy", [_p], None)
 _decl("molot_paged_decode_gather",
       [_p, _p, _p, ctypes.c_size_t, _p, _p, _p, _i, _i, _f, _p])
+
+class _F8LayerStruct(ctypes.Structure):
+    """molot_f8b_layer."""
+    _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p), ("weight", _p),
+                ("block_table", _p), ("max_pages", _i), ("page_size", _i)]
+
+
+_lp = ctypes.POINTER(_F8LayerStruct)
+_decl("molot_pager_layer_blocks", [_p, _i, _pp, _pp, _pp])
+_decl("molot_f8b_plan_create", [_pp])
+_decl("molot_f8b_plan_destroy", [_p], None)
+_decl("molot_f8b_plan_build", [_p, _i, _i, _i, _i, _p, _p, _p, _p, _i, _p])
+_decl("molot_f8b_write", [_p, _lp, _p, _p, _i, _ll, _ll, _p])
+_decl("molot_f8b_decode", [_p, _lp, _p, _p, _p, _i, _ll, _f, _f, _p, _p, _p])
+_decl("molot_f8b_evict", [_p, _lp, _lp, _i, _i, _p, _p])
+_decl("molot_packed_plan_create", [_pp])
+_decl("molot_packed_plan_destroy", [_p], None)
+_decl("molot_packed_plan_build", [_p, _i, _i, _i, _i, _p, _p, _p, _i, _p])
+_decl("molot_packed_attend", [_p, _p, _p, _p, _p, _p, _i, _ll, _ll, _ll, _f, _f, _p, _p])
 
 COMM_HANDLE_BYTES = 64
 COMM_MAX_RANKS = 8
@@ -488,11 +515,11 @@ class Pager:
 
     def __init__(self, n_layers, nkv, d, page_size, num_pages, max_seqs, max_pages_per_seq,
                  dtype: str = "f32"):
-        if dtype not in _KV_DTYPES:
-            raise ValueError("dtype must be 'f32', 'bf16' or 'q8'")
+        if dtype not in _POOL_DTYPES:
+            raise ValueError("dtype must be 'f32', 'bf16', 'q8' or 'f8b'")
         h = ctypes.c_void_p()
         check(_lib.molot_pager_create_ex(n_layers, nkv, d, page_size, num_pages, max_seqs,
-                                         max_pages_per_seq, _KV_DTYPES[dtype], ctypes.byref(h)))
+                                         max_pages_per_seq, _POOL_DTYPES[dtype], ctypes.byref(h)))
         self._h = h
         self.dtype = dtype
         self.n_layers, self.nkv, self.d, self.page_size = n_layers, nkv, d, page_size
@@ -540,14 +567,14 @@ class Pager:
     def layer_pools(self, layer: int):
         """(K, V) torch views [num_pages][nkv][page_size][d] of a layer's pools:
         float32, bfloat16 for bf16 pools, uint8 rows of q8_row_bytes(d) for
-        q8 pools."""
+        q8 pools, uint8 codes for f8b pools."""
         import torch
         k = ctypes.c_void_p()
         v = ctypes.c_void_p()
         check(_lib.molot_pager_layer_pools(self._h, layer, ctypes.byref(k), ctypes.byref(v)))
         shape = (self.num_pages, self.nkv, self.page_size, self.d)
-        if self.dtype == "q8":
-            shape = shape[:3] + (q8_row_bytes(self.d),)
+        if self.dtype in ("q8", "f8b"):
+            shape = shape[:3] + (q8_row_bytes(self.d) if self.dtype == "q8" else self.d,)
             return (torch.as_tensor(_CudaArray(k.value, shape, "|u1"), device="cuda"),
                     torch.as_tensor(_CudaArray(v.value, shape, "|u1"), device="cuda"))
         if self.dtype == "bf16":
@@ -557,6 +584,25 @@ class Pager:
                                     device="cuda").view(torch.bfloat16))
         return (torch.as_tensor(_CudaArray(k.value, shape), device="cuda"),
                 torch.as_tensor(_CudaArray(v.value, shape), device="cuda"))
+
+    def layer_blocks(self, layer: int):
+        """(k_scale, v_scale, weight) torch views of a layer of f8b pools:
+        scales [num_pages][nkv][page_size/16], counters
+        [num_pages][nkv][page_size]."""
+        import torch
+        ks, vs, w = ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_void_p()
+        check(_lib.molot_pager_layer_blocks(self._h, layer, ctypes.byref(ks), ctypes.byref(vs),
+                                            ctypes.byref(w)))
+        shape = (self.num_pages, self.nkv, self.page_size // 16)
+        return (torch.as_tensor(_CudaArray(ks.value, shape), device="cuda"),
+                torch.as_tensor(_CudaArray(vs.value, shape), device="cuda"),
+                torch.as_tensor(_CudaArray(w.value, shape[:2] + (self.page_size,)), device="cuda"))
+
+    def f8_layer(self, layer: int, block_table) -> "F8Layer":
+        """The layer's f8b pools with a batch's block table (a CUDA tensor)."""
+        k, v = self.layer_pools(layer)
+        ks, vs, w = self.layer_blocks(layer)
+        return F8Layer(k, v, ks, vs, block_table, weight=w)
 
 
 class PagedPlan:
@@ -612,6 +658,187 @@ class PagedPlan:
 
     def check(self, stream=None) -> None:
         check(_lib.molot_paged_check(self._h, _stream_ptr(stream)))
+
+
+def _cuda_f32(t, name, shape=None):
+    _check_cuda_tensor(t, name)
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}")
+    return t.data_ptr()
+
+
+def _rows(t, name, n, heads, d, act=None):
+    """Pointer, row stride and molot_act_dtype of rows [n][heads][d] whose
+    heads are contiguous (a part of a wider projection's rows will do)."""
+    if not (hasattr(t, "is_cuda") and t.is_cuda):
+        raise ValueError(f"{name} must be a CUDA tensor")
+    ty = _ACT_DTYPES.get(str(t.dtype))
+    if ty is None or (act is not None and ty != act):
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, like the other operands")
+    if tuple(t.shape) != (n, heads, d):
+        raise ValueError(f"{name} must have shape {(n, heads, d)}")
+    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != d):
+        raise ValueError(f"{name} must have contiguous heads")
+    return t.data_ptr(), t.stride(0) if n > 1 else heads * d, ty
+
+
+class F8Layer:
+    """One layer of 8-bit block-scaled pools: codes [pages][nkv][page_size][d]
+    uint8, scales [pages][nkv][page_size/16] float32, optionally counters
+    [pages][nkv][page_size] float32, and a batch's block table
+    [B][max_pages] int32, all contiguous CUDA tensors."""
+
+    def __init__(self, k, v, k_scale, v_scale, block_table, weight=None):
+        pages, nkv, ps, d = k.shape
+        for t, name in ((k, "k"), (v, "v")):
+            if not t.is_cuda or str(t.dtype) != "torch.uint8" or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous uint8 CUDA tensor")
+        if v.shape != k.shape:
+            raise ValueError("k and v must have one shape")
+        if not block_table.is_cuda or str(block_table.dtype) != "torch.int32" or \
+                not block_table.is_contiguous() or block_table.dim() != 2:
+            raise ValueError("block_table must be a contiguous int32 CUDA tensor [B][max_pages]")
+        self.tensors = (k, v, k_scale, v_scale, weight, block_table)  # kept alive
+        self.nkv, self.page_size, self.d = nkv, ps, d
+        self.batch, self.max_pages = block_table.shape
+        self.weight_shape = (pages, nkv, ps)
+        sc = (pages, nkv, ps // 16)
+        self._s = _F8LayerStruct(
+            k.data_ptr(), v.data_ptr(), _cuda_f32(k_scale, "k_scale", sc),
+            _cuda_f32(v_scale, "v_scale", sc),
+            None if weight is None else _cuda_f32(weight, "weight", self.weight_shape),
+            block_table.data_ptr(), self.max_pages, ps)
+
+
+class F8Plan:
+    """Batch of one step over 8-bit block-scaled pools (molot_f8b_*)."""
+
+    def __init__(self):
+        h = ctypes.c_void_p()
+        check(_lib.molot_f8b_plan_create(ctypes.byref(h)))
+        self._h = h
+        self.B = 0
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            _lib.molot_f8b_plan_destroy(self._h)
+            self._h = None
+
+    def __del__(self):  # pragma: no cover
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def build(self, nq, nkv, d, seq_lens, new_lens=None, starts=None, prefix=None, window=0,
+              stream=None) -> None:
+        arrays = []
+        for a in (seq_lens, new_lens, starts, prefix):
+            a = None if a is None else np.ascontiguousarray(a, dtype=np.int32)
+            if a is not None and a.shape != (len(seq_lens),):
+                raise ValueError("one entry per sequence")
+            arrays.append(a)
+        self.B = 0  # until it is built
+        check(_lib.molot_f8b_plan_build(self._h, arrays[0].size, nq, nkv, d,
+                                        *(_ptr(a) for a in arrays), window, _stream_ptr(stream)))
+        self.B, self.nq, self.nkv, self.d = arrays[0].size, nq, nkv, d
+        self.rows = int(np.minimum(arrays[0], 1).sum() if arrays[1] is None else arrays[1].sum())
+
+    def _layer(self, layer, name="layer"):
+        if not self.B:
+            raise ValueError("plan not built")
+        if (layer.nkv, layer.d) != (self.nkv, self.d) or layer.batch != self.B:
+            raise ValueError(f"{name} does not fit the plan's heads or batch")
+        return ctypes.byref(layer._s)
+
+    def write(self, layer, k, v, stream=None) -> None:
+        """k, v [new rows][nkv][d] float32, bfloat16 or float16."""
+        lp = self._layer(layer)
+        kp, ks, ty = _rows(k, "k", self.rows, self.nkv, self.d)
+        vp, vs, _ = _rows(v, "v", self.rows, self.nkv, self.d, ty)
+        check(_lib.molot_f8b_write(self._h, lp, kp, vp, ty, ks, vs, _stream_ptr(stream)))
+
+    def decode(self, layer, q, o, scale, softcap=0.0, slopes=None, lse=None, weight_out=None,
+               stream=None) -> None:
+        """q, o [B][nq][d]; slopes [nq], lse [B][nq] float32; weight_out a
+        counter pool like the layer's (itself allowed)."""
+        lp = self._layer(layer)
+        qp, qs, ty = _rows(q, "q", self.B, self.nq, self.d)
+        op, _, _ = _rows(o, "o", self.B, self.nq, self.d, ty)
+        if not o.is_contiguous():
+            raise ValueError("o must be contiguous")
+        check(_lib.molot_f8b_decode(
+            self._h, lp, qp, op, None if lse is None else _cuda_f32(lse, "lse", (self.B, self.nq)),
+            ty, qs, scale, softcap,
+            None if slopes is None else _cuda_f32(slopes, "slopes", (self.nq,)),
+            None if weight_out is None else _cuda_f32(weight_out, "weight_out",
+                                                      layer.weight_shape),
+            _stream_ptr(stream)))
+
+    def evict(self, src, dst, budget, recent, kept, stream=None) -> None:
+        """Moves the slots to keep from src to dst (pages of its own);
+        kept [B][nkv][budget] int32 receives the source slots."""
+        sp, dp = self._layer(src, "src"), self._layer(dst, "dst")
+        if not kept.is_cuda or str(kept.dtype) != "torch.int32" or not kept.is_contiguous() or \
+                tuple(kept.shape) != (self.B, self.nkv, budget):
+            raise ValueError("kept must be a contiguous int32 CUDA tensor [B][nkv][budget]")
+        check(_lib.molot_f8b_evict(self._h, sp, dp, budget, recent, kept.data_ptr(),
+                                   _stream_ptr(stream)))
+
+
+class PackedPlan:
+    """Prefill attention over packed documents (molot_packed_*)."""
+
+    def __init__(self):
+        h = ctypes.c_void_p()
+        check(_lib.molot_packed_plan_create(ctypes.byref(h)))
+        self._h = h
+        self.ndocs = 0
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            _lib.molot_packed_plan_destroy(self._h)
+            self._h = None
+
+    def __del__(self):  # pragma: no cover
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def build(self, nq, nkv, d, q_lens, k_lens=None, prefix=None, window=0, stream=None) -> None:
+        arrays = []
+        for a in (q_lens, k_lens, prefix):
+            a = None if a is None else np.ascontiguousarray(a, dtype=np.int32)
+            if a is not None and a.shape != (len(q_lens),):
+                raise ValueError("one entry per document")
+            arrays.append(a)
+        self.ndocs = 0  # until it is built
+        check(_lib.molot_packed_plan_build(self._h, arrays[0].size, nq, nkv, d,
+                                           *(_ptr(a) for a in arrays), window,
+                                           _stream_ptr(stream)))
+        self.ndocs, self.nq, self.nkv, self.d = arrays[0].size, nq, nkv, d
+        self.rows = int(arrays[0].sum())
+        self.keys = self.rows if arrays[1] is None else int(arrays[1].sum())
+
+    def attend(self, q, k, v, o, scale, softcap=0.0, slopes=None, lse=None, stream=None) -> None:
+        """q, o [rows][nq][d], k, v [keys][nkv][d] bfloat16 or float16;
+        slopes [nq], lse [rows][nq] float32."""
+        if not self.ndocs:
+            raise ValueError("plan not built")
+        qp, qs, ty = _rows(q, "q", self.rows, self.nq, self.d)
+        kp, ks, _ = _rows(k, "k", self.keys, self.nkv, self.d, ty)
+        vp, vs, _ = _rows(v, "v", self.keys, self.nkv, self.d, ty)
+        op, _, _ = _rows(o, "o", self.rows, self.nq, self.d, ty)
+        if not o.is_contiguous():
+            raise ValueError("o must be contiguous")
+        check(_lib.molot_packed_attend(
+            self._h, qp, kp, vp, op,
+            None if lse is None else _cuda_f32(lse, "lse", (self.rows, self.nq)), ty, qs, ks, vs,
+            scale, softcap, None if slopes is None else _cuda_f32(slopes, "slopes", (self.nq,)),
+            _stream_ptr(stream)))
 
 
 class Comm:

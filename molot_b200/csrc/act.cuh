@@ -1,0 +1,101 @@
+// Pieces that the kernels of the 8-bit cache and of packed attention share:
+// activation types, warp helpers and the modified scores.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math_constants.h>
+
+#include <cstdint>
+
+namespace molot {
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a <= 3.402823466e38f ? a : 0.f;  // infinities and NaN do not set a scale
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Row types: EPL elements in 16 bytes.
+template <class T>
+struct Act;
+template <>
+struct Act<float> {
+  static constexpr int EPL = 4;
+  __device__ static void load(const float* p, float* x) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  }
+  __device__ static float one(const float* p) { return *p; }
+  __device__ static void store(float* p, float x) { *p = x; }
+};
+template <>
+struct Act<__nv_bfloat16> {
+  static constexpr int EPL = 8;
+  __device__ static void load(const __nv_bfloat16* p, float* x) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  __device__ static float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  __device__ static void store(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+};
+template <>
+struct Act<__half> {
+  static constexpr int EPL = 8;
+  __device__ static void load(const __half* p, float* x) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+  __device__ static float one(const __half* p) { return __half2float(*p); }
+  __device__ static void store(__half* p, float x) { *p = __float2half_rn(x); }
+};
+
+// Index of the interval of prefix[0..n] (ascending, prefix[0] = 0) that holds
+// x, 0 <= x < prefix[n]: a search by the whole warp, 32 probes at a time, so
+// two dependent loads serve 1024 intervals.
+__device__ __forceinline__ int warp_find(const int* __restrict__ prefix, int n, int x) {
+  int lo = 0, len = n;  // the answer is in [lo, lo + len)
+  const int lane = threadIdx.x & 31;
+  while (len > 1) {
+    const int step = (len + 31) / 32;
+    const int i = lo + (lane + 1) * step;  // probe: is prefix[i] <= x ?
+    const bool le = i < lo + len && prefix[i] <= x;
+    const int k = __popc(__ballot_sync(0xffffffffu, le));
+    lo += k * step;
+    len = min(step, len - k * step);
+  }
+  return lo;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Score q.k * scale -> base-2 logit: cap, distance bias (dist = newest - slot).
+__device__ __forceinline__ float score_logit(float s, float cap, float slope, float dist) {
+  if (cap > 0.f) s = cap * tanhf(s / cap);
+  return (s - slope * dist) * kLog2e;
+}
+
+}  // namespace molot

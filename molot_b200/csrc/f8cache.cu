@@ -1,0 +1,341 @@
+// C ABI of the 8-bit block-scaled paged cache (molot_f8b_*): plans, argument
+// checks, scratch and launches.
+#include "f8cache.cuh"
+
+#include <algorithm>
+#include <cstdio>
+#include <cstring>
+#include <new>
+#include <type_traits>
+#include <vector>
+
+#include "molot_b200.h"
+
+namespace molot {
+int set_last_error(int code, const char* msg);
+
+namespace {
+
+int f8_fail(int code, const char* msg) { return set_last_error(code, msg); }
+
+int f8_cuda(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return MOLOT_OK;
+  char buf[256];
+  snprintf(buf, sizeof buf, "%s: %s", what, cudaGetErrorString(e));
+  return set_last_error(e == cudaErrorMemoryAllocation ? MOLOT_ERR_NOMEM : MOLOT_ERR_CUDA, buf);
+}
+
+#define F8_CUDA(call)                                  \
+  do {                                                 \
+    if (int rc_ = f8_cuda((call), #call)) return rc_;  \
+  } while (0)
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+size_t act_bytes(int t) { return t == MOLOT_ACT_F32 ? 4 : 2; }
+
+// f(T{}, D) for an activation type and a head size.
+template <class F>
+int f8_dispatch(int act, int d, F&& f) {
+  auto by_d = [&](auto t) {
+    switch (d) {
+      case 64: return f(t, std::integral_constant<int, 64>{});
+      case 128: return f(t, std::integral_constant<int, 128>{});
+      default: return f(t, std::integral_constant<int, 256>{});
+    }
+  };
+  switch (act) {
+    case MOLOT_ACT_F32: return by_d(float{});
+    case MOLOT_ACT_BF16: return by_d(__nv_bfloat16{});
+    default: return by_d(__half{});
+  }
+}
+
+}  // namespace
+}  // namespace molot
+
+using namespace molot;
+
+struct molot_f8b_plan {
+  int device = -1;
+  bool built = false;
+  int B = 0, nq = 0, nkv = 0, d = 0;
+  int max_len = 0, max_end = 0;  // longest sequence
+  int rows = 0, touched = 0;     // new rows, blocks they touch
+  long long visits = 0;          // block visits of a decode (per kv head)
+  int* h_buf = nullptr;          // pinned staging
+  int* d_buf = nullptr;
+  size_t h_cap = 0, d_cap = 0;  // ints
+  cudaEvent_t uploaded = nullptr;
+  size_t o_prefix = 0, o_n0 = 0, o_len = 0, o_row = 0, o_blk = 0;  // F8Seq first
+  float* score = nullptr;  // accumulation scratch: scores, then [B][nq] lse
+  size_t score_cap = 0;
+
+  const F8Seq* seqs() const { return reinterpret_cast<const F8Seq*>(d_buf); }
+};
+
+namespace molot {
+namespace {
+
+int f8_build(molot_f8b_plan* p, int B, int nq, int nkv, int d, const int* seq_lens,
+             const int* new_lens, const int* starts, const int* prefix, int window,
+             cudaStream_t st) {
+  std::vector<F8Seq> seqs(B);
+  std::vector<int> visit(B + 1), n0(B), len(B), row(B + 1), blk(B + 1);
+  long long nv = 0, nr = 0, nb = 0;
+  int max_len = 0;
+  for (int b = 0; b < B; ++b) {
+    const int n = seq_lens[b];
+    if (n < 0 || n > (1 << 30)) return f8_fail(MOLOT_ERR_INVALID, "sequence length out of range");
+    const int m = new_lens ? new_lens[b] : std::min(n, 1);
+    if (m < 0 || m > n) return f8_fail(MOLOT_ERR_INVALID, "new_lens must be within [0, length]");
+    const int first = starts ? starts[b] : 0;
+    if (first < 0 || first > n) return f8_fail(MOLOT_ERR_INVALID, "starts must be within [0, length]");
+    const int pre = prefix ? prefix[b] : 0;
+    if (pre < 0) return f8_fail(MOLOT_ERR_INVALID, "negative prefix");
+    F8Seq& s = seqs[b];
+    s = F8Seq{};
+    s.n = n;
+    s.first = first;
+    s.lo = window > 0 ? std::max(first, n - window) : first;
+    s.sink_end = (int)std::min<long long>(n, (long long)first + pre);
+    if (n > first) {
+      s.b0 = s.lo / kF8Blk;
+      s.a0 = first / kF8Blk;
+      const int a1 = s.sink_end > first ? (s.sink_end + kF8Blk - 1) / kF8Blk : s.a0;
+      s.na = std::max(0, std::min(a1, s.b0) - s.a0);
+      s.nblk = s.na + (n + kF8Blk - 1) / kF8Blk - s.b0;
+    }
+    visit[b] = (int)nv;
+    nv += (long long)s.nblk * nkv;
+    n0[b] = n - m;
+    len[b] = n;
+    row[b] = (int)nr;
+    nr += m;
+    blk[b] = (int)nb;
+    nb += m > 0 ? (n + kF8Blk - 1) / kF8Blk - (n - m) / kF8Blk : 0;
+    if (nv > 0x7fffffff || nr > 0x7fffffff || nb * nkv * 2 > 0x7fffffff)
+      return f8_fail(MOLOT_ERR_INVALID, "batch too large");
+    max_len = std::max(max_len, n);
+  }
+  visit[B] = (int)nv;
+  row[B] = (int)nr;
+  blk[B] = (int)nb;
+  const size_t o_prefix = (size_t)B * (sizeof(F8Seq) / 4), o_n0 = o_prefix + B + 1,
+               o_len = o_n0 + B, o_row = o_len + B, o_blk = o_row + B + 1,
+               total = o_blk + B + 1;
+  if (p->built) F8_CUDA(cudaEventSynchronize(p->uploaded));  // staging still being read?
+  p->built = false;
+  if (p->h_cap < total) {
+    if (p->h_buf) cudaFreeHost(p->h_buf);
+    p->h_buf = nullptr;
+    p->h_cap = 0;
+    F8_CUDA(cudaMallocHost(&p->h_buf, total * sizeof(int)));
+    p->h_cap = total;
+  }
+  if (p->d_cap < total) {
+    F8_CUDA(cudaDeviceSynchronize());
+    cudaFree(p->d_buf);
+    p->d_buf = nullptr;
+    p->d_cap = 0;
+    const size_t cap = std::max<size_t>(total, 1024);
+    F8_CUDA(cudaMalloc(&p->d_buf, cap * sizeof(int)));
+    p->d_cap = cap;
+  }
+  std::memcpy(p->h_buf, seqs.data(), B * sizeof(F8Seq));
+  std::memcpy(p->h_buf + o_prefix, visit.data(), (B + 1) * sizeof(int));
+  std::memcpy(p->h_buf + o_n0, n0.data(), B * sizeof(int));
+  std::memcpy(p->h_buf + o_len, len.data(), B * sizeof(int));
+  std::memcpy(p->h_buf + o_row, row.data(), (B + 1) * sizeof(int));
+  std::memcpy(p->h_buf + o_blk, blk.data(), (B + 1) * sizeof(int));
+  F8_CUDA(cudaMemcpyAsync(p->d_buf, p->h_buf, total * sizeof(int), cudaMemcpyHostToDevice, st));
+  F8_CUDA(cudaEventRecord(p->uploaded, st));
+  p->o_prefix = o_prefix;
+  p->o_n0 = o_n0;
+  p->o_len = o_len;
+  p->o_row = o_row;
+  p->o_blk = o_blk;
+  p->B = B;
+  p->nq = nq;
+  p->nkv = nkv;
+  p->d = d;
+  p->max_len = max_len;
+  p->rows = (int)nr;
+  p->touched = (int)nb;
+  p->visits = nv;
+  p->built = true;
+  return MOLOT_OK;
+}
+
+// Checks a layer's pools for slots [0, max_len) of every sequence.
+int f8_pool(const molot_f8b_plan* p, const molot_f8b_layer* l, int max_len, F8Pool* out) {
+  if (!p || !p->built) return f8_fail(MOLOT_ERR_INVALID, "plan not built");
+  if (!l || !l->k || !l->v || !l->k_scale || !l->v_scale || !l->block_table)
+    return f8_fail(MOLOT_ERR_INVALID, "null pointer");
+  if (!aligned16(l->k) || !aligned16(l->v))
+    return f8_fail(MOLOT_ERR_INVALID, "code pools must be 16-byte aligned");
+  if (l->page_size <= 0 || l->page_size % kF8Blk)
+    return f8_fail(MOLOT_ERR_INVALID, "page_size must be a multiple of 16");
+  if ((long long)l->max_pages * l->page_size < max_len)
+    return f8_fail(MOLOT_ERR_INVALID, "block table too narrow for the plan's sequences");
+  int dev = -1;
+  F8_CUDA(cudaGetDevice(&dev));
+  if (dev != p->device) return f8_fail(MOLOT_ERR_INVALID, "plan used on another device");
+  *out = F8Pool{static_cast<uint8_t*>(l->k), static_cast<uint8_t*>(l->v), l->k_scale, l->v_scale,
+                l->block_table, l->max_pages, l->page_size, p->nkv, p->d};
+  return MOLOT_OK;
+}
+
+}  // namespace
+}  // namespace molot
+
+extern "C" {
+
+int molot_f8b_plan_create(molot_f8b_plan** out) {
+  if (!out) return f8_fail(MOLOT_ERR_INVALID, "null out");
+  *out = nullptr;
+  int n = 0, dev = 0;
+  if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0)
+    return f8_fail(MOLOT_ERR_NO_DEVICE, "no CUDA device visible");
+  F8_CUDA(cudaGetDevice(&dev));
+  auto* p = new (std::nothrow) molot_f8b_plan();
+  if (!p) return f8_fail(MOLOT_ERR_NOMEM, "plan");
+  p->device = dev;
+  if (int rc = f8_cuda(cudaEventCreateWithFlags(&p->uploaded, cudaEventDisableTiming),
+                       "cudaEventCreate")) {
+    delete p;
+    return rc;
+  }
+  *out = p;
+  return MOLOT_OK;
+}
+
+void molot_f8b_plan_destroy(molot_f8b_plan* p) {
+  if (!p) return;
+  int prev = -1;
+  cudaGetDevice(&prev);
+  cudaSetDevice(p->device);
+  cudaDeviceSynchronize();
+  cudaFreeHost(p->h_buf);
+  cudaFree(p->d_buf);
+  cudaFree(p->score);
+  cudaEventDestroy(p->uploaded);
+  if (prev >= 0) cudaSetDevice(prev);
+  delete p;
+}
+
+int molot_f8b_plan_build(molot_f8b_plan* p, int B, int nq, int nkv, int d, const int* seq_lens,
+                         const int* new_lens, const int* starts, const int* prefix, int window,
+                         void* stream) {
+  if (!p || !seq_lens || B <= 0 || B > 65535) return f8_fail(MOLOT_ERR_INVALID, "bad plan arguments");
+  if (nq <= 0 || nkv <= 0 || nkv > 65535 || nq % nkv)
+    return f8_fail(MOLOT_ERR_INVALID, "nq must be a multiple of nkv");
+  if (d != 64 && d != 128 && d != 256)
+    return f8_fail(MOLOT_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256");
+  if (nq / nkv > 64) return f8_fail(MOLOT_ERR_UNSUPPORTED, "nq / nkv must be at most 64");
+  int dev = -1;
+  F8_CUDA(cudaGetDevice(&dev));
+  if (dev != p->device) return f8_fail(MOLOT_ERR_INVALID, "plan used on another device");
+  try {
+    return f8_build(p, B, nq, nkv, d, seq_lens, new_lens, starts, prefix, window,
+                    (cudaStream_t)stream);
+  } catch (const std::exception&) {
+    return f8_fail(MOLOT_ERR_NOMEM, "plan arrays");
+  }
+}
+
+int molot_f8b_write(molot_f8b_plan* p, const molot_f8b_layer* layer, const void* k, const void* v,
+                    int act_dtype, long long k_stride, long long v_stride, void* stream) {
+  F8Pool pool;
+  if (int rc = f8_pool(p, layer, p ? p->max_len : 0, &pool)) return rc;
+  if (act_dtype < MOLOT_ACT_F32 || act_dtype > MOLOT_ACT_F16)
+    return f8_fail(MOLOT_ERR_INVALID, "unknown act_dtype");
+  if (p->rows == 0) return MOLOT_OK;
+  if (!k || !v) return f8_fail(MOLOT_ERR_INVALID, "null pointer");
+  const size_t es = act_bytes(act_dtype);
+  if (k_stride < (long long)p->nkv * p->d || v_stride < (long long)p->nkv * p->d ||
+      k_stride * es % 16 || v_stride * es % 16 || !aligned16(k) || !aligned16(v))
+    return f8_fail(MOLOT_ERR_INVALID,
+                   "rows must be 16-byte aligned and at least nkv * d elements apart");
+  const F8WriteArgs a{pool, k, v, k_stride, v_stride, p->d_buf + p->o_n0, p->d_buf + p->o_len,
+                      p->d_buf + p->o_row, p->d_buf + p->o_blk, layer->weight, p->B, p->touched * p->nkv * 2};
+  return f8_dispatch(act_dtype, p->d, [&](auto t, auto dd) {
+    f8_write_kernel<decltype(t), decltype(dd)::value>
+        <<<(a.nitems + 3) / 4, 128, 0, (cudaStream_t)stream>>>(a);
+    return f8_cuda(cudaGetLastError(), "f8 write launch");
+  });
+}
+
+int molot_f8b_decode(molot_f8b_plan* p, const molot_f8b_layer* layer, const void* q, void* o,
+                     float* lse, int act_dtype, long long q_stride, float scale, float softcap,
+                     const float* slopes, float* weight_out, void* stream) {
+  F8Pool pool;
+  if (int rc = f8_pool(p, layer, p ? p->max_len : 0, &pool)) return rc;
+  if (act_dtype < MOLOT_ACT_F32 || act_dtype > MOLOT_ACT_F16)
+    return f8_fail(MOLOT_ERR_INVALID, "unknown act_dtype");
+  if (!q || !o) return f8_fail(MOLOT_ERR_INVALID, "null pointer");
+  if (q_stride < (long long)p->nq * p->d || q_stride * act_bytes(act_dtype) % 16 || !aligned16(q) ||
+      !aligned16(o))
+    return f8_fail(MOLOT_ERR_INVALID, "q and o must be 16-byte aligned, q_stride at least nq * d");
+  if (!(softcap >= 0.f) || softcap > 3e38f || !(scale == scale))
+    return f8_fail(MOLOT_ERR_INVALID, "softcap must be finite and not negative");
+  if (weight_out && !layer->weight)
+    return f8_fail(MOLOT_ERR_INVALID, "weight_out needs the layer's weight");
+  const int G = p->nq / p->nkv;
+  float* lse2 = nullptr;
+  if (weight_out) {
+    const size_t ns = (size_t)p->visits * kF8Blk * G, need = ns + (size_t)p->B * p->nq;
+    if (need > p->score_cap) {
+      F8_CUDA(cudaDeviceSynchronize());
+      cudaFree(p->score);
+      p->score = nullptr;
+      p->score_cap = 0;
+      F8_CUDA(cudaMalloc(&p->score, need * sizeof(float)));
+      p->score_cap = need;
+    }
+    lse2 = p->score + ns;
+  }
+  const F8DecodeArgs a{pool, p->seqs(), p->d_buf + p->o_prefix, q, o, lse,
+                       weight_out ? p->score : nullptr, lse2, slopes, q_stride, p->B, p->nq, G,
+                       scale, softcap};
+  if (int rc = f8_dispatch(act_dtype, p->d, [&](auto t, auto dd) {
+        f8_decode_kernel<decltype(t), decltype(dd)::value>
+            <<<dim3(p->nq, p->B), 128, 0, (cudaStream_t)stream>>>(a);
+        return f8_cuda(cudaGetLastError(), "f8 decode launch");
+      }))
+    return rc;
+  if (!weight_out || !p->max_len) return MOLOT_OK;
+  const F8WeightArgs w{pool, p->seqs(), p->d_buf + p->o_prefix, p->score, lse2, layer->weight,
+                       weight_out, p->nq, G};
+  f8_weight_kernel<<<dim3((p->max_len + 127) / 128, p->nkv, p->B), 128, 0, (cudaStream_t)stream>>>(w);
+  return f8_cuda(cudaGetLastError(), "f8 weight launch");
+}
+
+int molot_f8b_evict(molot_f8b_plan* p, const molot_f8b_layer* src, const molot_f8b_layer* dst,
+                    int budget, int recent, int* kept, void* stream) {
+  if (budget <= 0 || recent < 0 || recent > budget)
+    return f8_fail(MOLOT_ERR_INVALID, "need 0 <= recent <= budget and budget > 0");
+  F8EvictArgs a{};
+  if (int rc = f8_pool(p, src, p ? p->max_len : 0, &a.src)) return rc;
+  if (int rc = f8_pool(p, dst, std::min(p->max_len, budget), &a.dst)) return rc;
+  if (!src->weight || !dst->weight || !kept) return f8_fail(MOLOT_ERR_INVALID, "null pointer");
+  a.win = src->weight;
+  a.wout = dst->weight;
+  a.kept = kept;
+  a.seqs = p->seqs();
+  a.B = p->B;
+  a.budget = budget;
+  a.recent = recent;
+  f8_select_kernel<<<dim3(p->nkv, p->B), kF8SelThreads, 0, (cudaStream_t)stream>>>(a);
+  F8_CUDA(cudaGetLastError());
+  const int blocks = (std::min(p->max_len, budget) + kF8Blk - 1) / kF8Blk;
+  if (!blocks) return MOLOT_OK;
+  const dim3 grid((blocks * p->nkv * 2 + 3) / 4, p->B);
+  switch (p->d) {
+    case 64: f8_move_kernel<64><<<grid, 128, 0, (cudaStream_t)stream>>>(a); break;
+    case 128: f8_move_kernel<128><<<grid, 128, 0, (cudaStream_t)stream>>>(a); break;
+    default: f8_move_kernel<256><<<grid, 128, 0, (cudaStream_t)stream>>>(a); break;
+  }
+  return f8_cuda(cudaGetLastError(), "f8 move launch");
+}
+
+}  // extern "C"

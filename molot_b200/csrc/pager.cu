@@ -31,6 +31,8 @@ struct molot_pager {
   std::vector<char> live;
   unsigned char* pools = nullptr;  // [n_layers][2][num_pages][nkv][page_size][row], may be null
   size_t pool_bytes = 0;           // per K (or V) pool of one layer
+  unsigned char* blocks = nullptr;  // MOLOT_KV_F8B: [n_layers][k scales, v scales, counters]
+  size_t scale_bytes = 0, weight_bytes = 0;  // per layer
   int kvt = MOLOT_KV_F32;
   int device = -1;
   mutable std::mutex mu;  // every call, queries included
@@ -72,10 +74,14 @@ int molot_pager_create(int n_layers, int nkv, int d, int page_size, int num_page
 int molot_pager_create_ex(int n_layers, int nkv, int d, int page_size, int num_pages,
                           int max_seqs, int max_pages_per_seq, int kv_dtype, molot_pager** out) {
   if (!out) return pager_fail(MOLOT_ERR_INVALID, "null out");
-  if (kv_dtype != MOLOT_KV_F32 && kv_dtype != MOLOT_KV_BF16 && kv_dtype != MOLOT_KV_Q8)
-    return pager_fail(MOLOT_ERR_INVALID, "kv_dtype must be MOLOT_KV_F32, MOLOT_KV_BF16 or MOLOT_KV_Q8");
+  if (kv_dtype != MOLOT_KV_F32 && kv_dtype != MOLOT_KV_BF16 && kv_dtype != MOLOT_KV_Q8 &&
+      kv_dtype != MOLOT_KV_F8B)
+    return pager_fail(MOLOT_ERR_INVALID,
+                      "kv_dtype must be MOLOT_KV_F32, MOLOT_KV_BF16, MOLOT_KV_Q8 or MOLOT_KV_F8B");
   if (kv_dtype == MOLOT_KV_Q8 && d % 64)
     return pager_fail(MOLOT_ERR_INVALID, "Q8 pools need d a multiple of 64");
+  if (kv_dtype == MOLOT_KV_F8B && d != 64 && d != 128 && d != 256)
+    return pager_fail(MOLOT_ERR_INVALID, "F8B pools need d 64, 128 or 256");
   *out = nullptr;
   if (n_layers < 0 || nkv <= 0 || d <= 0 || page_size <= 0 || page_size % 16 || num_pages <= 0 ||
       max_seqs <= 0 || max_pages_per_seq <= 0)
@@ -96,15 +102,31 @@ int molot_pager_create_ex(int n_layers, int nkv, int d, int page_size, int num_p
   p->live.assign(max_seqs, 0);
   if (n_layers > 0) {
     cudaGetDevice(&p->device);
-    // bytes of one row of one kv head: d floats, d bf16, or a Q8 row
-    const size_t row = kv_dtype == MOLOT_KV_Q8 ? (size_t)((d + d / 8 + 15) & ~15)
-                                               : (size_t)d * (kv_dtype == MOLOT_KV_BF16 ? 2 : 4);
+    // bytes of one row of one kv head: d floats, d bf16, a Q8 row, or d codes
+    const size_t row = kv_dtype == MOLOT_KV_Q8    ? (size_t)((d + d / 8 + 15) & ~15)
+                       : kv_dtype == MOLOT_KV_F8B ? (size_t)d
+                                                  : (size_t)d * (kv_dtype == MOLOT_KV_BF16 ? 2 : 4);
     p->pool_bytes = ((size_t)num_pages * nkv * page_size * row + 255) & ~size_t(255);
     const cudaError_t e = cudaMalloc(&p->pools, p->pool_bytes * 2 * (size_t)n_layers);
     if (e != cudaSuccess) {
       delete p;
       return pager_fail(MOLOT_ERR_NOMEM, std::string("cudaMalloc(page pools): ") +
                                              cudaGetErrorString(e));
+    }
+    if (kv_dtype == MOLOT_KV_F8B) {
+      const size_t slots = (size_t)num_pages * nkv * page_size;
+      p->scale_bytes = (slots / 16 * sizeof(float) + 255) & ~size_t(255);
+      p->weight_bytes = (slots * sizeof(float) + 255) & ~size_t(255);
+      const size_t all = (2 * p->scale_bytes + p->weight_bytes) * (size_t)n_layers;
+      cudaError_t eb = cudaMalloc(&p->blocks, all);
+      if (eb == cudaSuccess) eb = cudaMemset(p->blocks, 0, all);
+      if (eb != cudaSuccess) {
+        cudaFree(p->blocks);
+        cudaFree(p->pools);
+        delete p;
+        return pager_fail(MOLOT_ERR_NOMEM, std::string("cudaMalloc(block scales): ") +
+                                               cudaGetErrorString(eb));
+      }
     }
   }
   *out = p;
@@ -119,6 +141,7 @@ void molot_pager_destroy(molot_pager* p) {
     cudaSetDevice(p->device);
     cudaDeviceSynchronize();
     cudaFree(p->pools);
+    cudaFree(p->blocks);
     if (prev >= 0) cudaSetDevice(prev);
   }
   delete p;
@@ -206,6 +229,17 @@ int molot_pager_layer_pools(molot_pager* p, int layer, float** k_pool, float** v
     return pager_fail(MOLOT_ERR_INVALID, "bad layer (or a pager without pools)");
   if (k_pool) *k_pool = reinterpret_cast<float*>(p->pools + (size_t)(2 * layer) * p->pool_bytes);
   if (v_pool) *v_pool = reinterpret_cast<float*>(p->pools + (size_t)(2 * layer + 1) * p->pool_bytes);
+  return MOLOT_OK;
+}
+
+int molot_pager_layer_blocks(molot_pager* p, int layer, float** k_scale, float** v_scale,
+                             float** weight) {
+  if (!p || layer < 0 || layer >= p->n_layers || !p->blocks)
+    return pager_fail(MOLOT_ERR_INVALID, "bad layer (or a pager without MOLOT_KV_F8B pools)");
+  unsigned char* base = p->blocks + (2 * p->scale_bytes + p->weight_bytes) * (size_t)layer;
+  if (k_scale) *k_scale = reinterpret_cast<float*>(base);
+  if (v_scale) *v_scale = reinterpret_cast<float*>(base + p->scale_bytes);
+  if (weight) *weight = reinterpret_cast<float*>(base + 2 * p->scale_bytes);
   return MOLOT_OK;
 }
 
