@@ -30,6 +30,8 @@ int f8_cuda(cudaError_t e, const char* what) {
     if (int rc_ = f8_cuda((call), #call)) return rc_;  \
   } while (0)
 
+constexpr int kF8MaxCtas = 2;  // decode CTAs per SM
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 size_t act_bytes(int t) { return t == MOLOT_ACT_F32 ? 4 : 2; }
 
@@ -69,6 +71,12 @@ struct molot_f8b_plan {
   size_t o_prefix = 0, o_n0 = 0, o_len = 0, o_row = 0, o_blk = 0;  // F8Seq first
   float* score = nullptr;  // accumulation scratch: scores, then [B][nq] lse
   size_t score_cap = 0;
+  float* rec = nullptr;  // decode records, then tickets
+  size_t rec_cap = 0;    // floats
+  int* tickets = nullptr;
+  size_t tickets_cap = 0;
+  int sms = 0;
+  bool has_empty = false;
 
   const F8Seq* seqs() const { return reinterpret_cast<const F8Seq*>(d_buf); }
 };
@@ -83,6 +91,7 @@ int f8_build(molot_f8b_plan* p, int B, int nq, int nkv, int d, const int* seq_le
   std::vector<int> visit(B + 1), n0(B), len(B), row(B + 1), blk(B + 1);
   long long nv = 0, nr = 0, nb = 0;
   int max_len = 0;
+  bool has_empty = false;
   for (int b = 0; b < B; ++b) {
     const int n = seq_lens[b];
     if (n < 0 || n > (1 << 30)) return f8_fail(MOLOT_ERR_INVALID, "sequence length out of range");
@@ -105,6 +114,7 @@ int f8_build(molot_f8b_plan* p, int B, int nq, int nkv, int d, const int* seq_le
       s.na = std::max(0, std::min(a1, s.b0) - s.a0);
       s.nblk = s.na + (n + kF8Blk - 1) / kF8Blk - s.b0;
     }
+    has_empty |= s.nblk == 0;
     visit[b] = (int)nv;
     nv += (long long)s.nblk * nkv;
     n0[b] = n - m;
@@ -141,6 +151,28 @@ int f8_build(molot_f8b_plan* p, int B, int nq, int nkv, int d, const int* seq_le
     F8_CUDA(cudaMalloc(&p->d_buf, cap * sizeof(int)));
     p->d_cap = cap;
   }
+  // decode scratch: two records a CTA, a ticket per segment
+  const size_t rec = (size_t)2 * kF8MaxCtas * p->sms * (8 * (size_t)d + 16);
+  const size_t tickets = (size_t)B * nkv * ((nq / nkv + 7) / 8);
+  if (p->rec_cap < rec || p->tickets_cap < tickets) {
+    F8_CUDA(cudaDeviceSynchronize());
+    if (p->rec_cap < rec) {
+      cudaFree(p->rec);
+      p->rec = nullptr;
+      p->rec_cap = 0;
+      F8_CUDA(cudaMalloc(&p->rec, rec * sizeof(float)));
+      p->rec_cap = rec;
+    }
+    if (p->tickets_cap < tickets) {
+      cudaFree(p->tickets);
+      p->tickets = nullptr;
+      p->tickets_cap = 0;
+      const size_t cap = std::max<size_t>(tickets, 1024);
+      F8_CUDA(cudaMalloc(&p->tickets, cap * sizeof(int)));
+      F8_CUDA(cudaMemsetAsync(p->tickets, 0, cap * sizeof(int), st));
+      p->tickets_cap = cap;
+    }
+  }
   std::memcpy(p->h_buf, seqs.data(), B * sizeof(F8Seq));
   std::memcpy(p->h_buf + o_prefix, visit.data(), (B + 1) * sizeof(int));
   std::memcpy(p->h_buf + o_n0, n0.data(), B * sizeof(int));
@@ -162,6 +194,7 @@ int f8_build(molot_f8b_plan* p, int B, int nq, int nkv, int d, const int* seq_le
   p->rows = (int)nr;
   p->touched = (int)nb;
   p->visits = nv;
+  p->has_empty = has_empty;
   p->built = true;
   return MOLOT_OK;
 }
@@ -200,6 +233,8 @@ int molot_f8b_plan_create(molot_f8b_plan** out) {
   auto* p = new (std::nothrow) molot_f8b_plan();
   if (!p) return f8_fail(MOLOT_ERR_NOMEM, "plan");
   p->device = dev;
+  cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, dev);
+  p->sms = std::max(p->sms, 1);
   if (int rc = f8_cuda(cudaEventCreateWithFlags(&p->uploaded, cudaEventDisableTiming),
                        "cudaEventCreate")) {
     delete p;
@@ -218,6 +253,8 @@ void molot_f8b_plan_destroy(molot_f8b_plan* p) {
   cudaFreeHost(p->h_buf);
   cudaFree(p->d_buf);
   cudaFree(p->score);
+  cudaFree(p->rec);
+  cudaFree(p->tickets);
   cudaEventDestroy(p->uploaded);
   if (prev >= 0) cudaSetDevice(prev);
   delete p;
@@ -294,12 +331,37 @@ int molot_f8b_decode(molot_f8b_plan* p, const molot_f8b_layer* layer, const void
     }
     lse2 = p->score + ns;
   }
-  const F8DecodeArgs a{pool, p->seqs(), p->d_buf + p->o_prefix, q, o, lse,
-                       weight_out ? p->score : nullptr, lse2, slopes, q_stride, p->B, p->nq, G,
-                       scale, softcap};
+  F8DecodeArgs a{};
+  a.pool = pool;
+  a.seqs = p->seqs();
+  a.prefix = p->d_buf + p->o_prefix;
+  a.q = q;
+  a.o = o;
+  a.lse = lse;
+  a.score = weight_out ? p->score : nullptr;
+  a.lse2 = lse2;
+  a.slopes = slopes;
+  a.rec = p->rec;
+  a.tickets = p->tickets;
+  a.q_stride = q_stride;
+  a.B = p->B;
+  a.nq = p->nq;
+  a.G = G;
+  a.HG = (G + 7) / 8;
+  a.items = p->visits * a.HG;
+  a.has_empty = p->has_empty;
+  a.scale = scale;
+  a.cap = softcap;
   if (int rc = f8_dispatch(act_dtype, p->d, [&](auto t, auto dd) {
-        f8_decode_kernel<decltype(t), decltype(dd)::value>
-            <<<dim3(p->nq, p->B), 128, 0, (cudaStream_t)stream>>>(a);
+        using F = F8Dec<decltype(t), decltype(dd)::value>;
+        const auto kernel = f8_decode_kernel<decltype(t), decltype(dd)::value>;
+        if (F::kSmem > 48 * 1024)
+          F8_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       F::kSmem));
+        static_assert(F::kCtas <= kF8MaxCtas, "records");
+        const int grid = (int)std::max<long long>(
+            1, std::min<long long>(a.items, (long long)F::kCtas * p->sms));
+        kernel<<<grid, kF8Warps * 32, F::kSmem, (cudaStream_t)stream>>>(a);
         return f8_cuda(cudaGetLastError(), "f8 decode launch");
       }))
     return rc;
