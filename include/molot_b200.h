@@ -512,7 +512,7 @@ typedef struct molot_packed_plan molot_packed_plan;
 
 int molot_packed_plan_create(molot_packed_plan** out);
 void molot_packed_plan_destroy(molot_packed_plan* plan);
-/* Host arrays of ndocs.  d 64, 128 or 256. */
+/* Host arrays of ndocs.  d 64, 128 or 256; nq / nkv at most 128. */
 int molot_packed_plan_build(molot_packed_plan* plan, int ndocs, int nq, int nkv, int d,
                             const int* q_lens, const int* k_lens, const int* prefix, int window,
                             void* stream);
@@ -524,6 +524,9 @@ int molot_packed_attend(molot_packed_plan* plan, const void* q, const void* k, c
                         void* o, float* lse, int act_dtype, long long q_stride,
                         long long k_stride, long long v_stride, float scale, float softcap,
                         const float* slopes, void* stream);
+/* Synchronises `stream` and reports (then clears) a launch of the plan that
+ * gave up on a bounded wait: MOLOT_ERR_TIMEOUT, its outputs are garbage. */
+int molot_packed_check(molot_packed_plan* plan, void* stream);
 
 #ifdef __cplusplus
 }

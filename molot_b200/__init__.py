@@ -181,6 +181,7 @@ _decl("molot_f8b_evict", [_p, _lp, _lp, _i, _i, _p, _p])
 _decl("molot_packed_plan_create", [_pp])
 _decl("molot_packed_plan_destroy", [_p], None)
 _decl("molot_packed_plan_build", [_p, _i, _i, _i, _i, _p, _p, _p, _i, _p])
+_decl("molot_packed_check", [_p, _p])
 _decl("molot_packed_attend", [_p, _p, _p, _p, _p, _p, _i, _ll, _ll, _ll, _f, _f, _p, _p])
 
 COMM_HANDLE_BYTES = 64
@@ -839,6 +840,9 @@ class PackedPlan:
             None if lse is None else _cuda_f32(lse, "lse", (self.rows, self.nq)), ty, qs, ks, vs,
             scale, softcap, None if slopes is None else _cuda_f32(slopes, "slopes", (self.nq,)),
             _stream_ptr(stream)))
+
+    def check(self, stream=None) -> None:
+        check(_lib.molot_packed_check(self._h, _stream_ptr(stream)))
 
 
 class Comm:

@@ -1,11 +1,14 @@
 // C ABI of packed-document prefill attention (molot_packed_*).
 #include "packed.cuh"
 
+#include <cudaTypedefs.h>
+
 #include <algorithm>
 #include <cstdio>
 #include <cstring>
 #include <exception>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "molot_b200.h"
@@ -37,76 +40,137 @@ using namespace molot;
 struct molot_packed_plan {
   int device = -1;
   bool built = false;
-  int ndocs = 0, nq = 0, nkv = 0, d = 0, window = 0;
-  int rows = 0, keys = 0;
-  int* h_buf = nullptr;
-  int* d_buf = nullptr;
-  size_t h_cap = 0, d_cap = 0, o_row = 0;
+  int nq = 0, nkv = 0, d = 0, window = 0;
+  int rows = 0, keys = 0, items = 0;
+  PackedItem* h_buf = nullptr;  // pinned staging
+  PackedItem* d_buf = nullptr;
+  size_t h_cap = 0, d_cap = 0;
+  int* status = nullptr;
   cudaEvent_t uploaded = nullptr;
 };
 
 namespace molot {
 namespace {
 
+constexpr unsigned long long kPkWaitNs = 2000000000ull;  // 2 s per bounded wait
+
+// Row tiles of a CTA and keys of a tile, as the kernel has them.
+int pk_tiles(int d) { return d == 256 ? PackedShape<256>::kTiles : PackedShape<128>::kTiles; }
+int pk_bn(int d) { return d == 256 ? PackedShape<256>::BN : PackedShape<128>::BN; }
+
 int pk_build(molot_packed_plan* p, int ndocs, const int* q_lens, const int* k_lens,
              const int* prefix, int window, int nq, int nkv, int d, cudaStream_t st) {
-  std::vector<PackedDoc> docs(ndocs);
-  std::vector<int> row(ndocs + 1);
+  std::vector<std::pair<int, PackedItem>> items;  // with their key tiles
+  const int bp = 128 / (nq / nkv), step = bp * pk_tiles(d), bn = pk_bn(d);
   long long q0 = 0, k0 = 0;
   for (int i = 0; i < ndocs; ++i) {
     const int ql = q_lens[i], kl = k_lens ? k_lens[i] : ql, pre = prefix ? prefix[i] : 0;
     if (ql < 0 || kl < 0 || pre < 0) return pk_fail(MOLOT_ERR_INVALID, "negative length or prefix");
-    docs[i] = PackedDoc{(int)q0, ql, (int)k0, kl, std::min(pre, kl), {0, 0, 0}};
-    row[i] = (int)q0;
+    if (q0 + ql > (1 << 30) || k0 + kl > (1 << 30))
+      return pk_fail(MOLOT_ERR_INVALID, "batch too large");
+    for (int m = 0; m < ql; m += step) {
+      const PackedItem it{(int)q0, m, ql, (int)k0, kl, std::min(pre, kl), {0, 0}};
+      const int first = kl - ql + m, last = kl - ql + std::min(m + step, ql) - 1;
+      const int lo = window > 0 ? std::max(0, first - window + 1) : 0;
+      const int hi = std::max(last + 1, it.prefix);
+      const int skip = std::max(0, lo / bn - (it.prefix + bn - 1) / bn);
+      items.emplace_back(std::max(0, (hi + bn - 1) / bn - skip), it);
+    }
     q0 += ql;
     k0 += kl;
-    if (q0 > (1 << 30) || k0 > (1 << 30)) return pk_fail(MOLOT_ERR_INVALID, "batch too large");
   }
-  row[ndocs] = (int)q0;
-  const size_t o_row = (size_t)ndocs * (sizeof(PackedDoc) / 4), total = o_row + ndocs + 1;
+  if (items.size() * (size_t)nkv > 0x7fffffff) return pk_fail(MOLOT_ERR_INVALID, "batch too large");
+  // the longest items first: CTAs start in this order
+  std::stable_sort(items.begin(), items.end(),
+                   [](const auto& x, const auto& y) { return x.first > y.first; });
   if (p->built) PK_CUDA(cudaEventSynchronize(p->uploaded));
   p->built = false;
-  if (p->h_cap < total) {
+  const size_t n = items.size();
+  if (p->h_cap < n) {
     cudaFreeHost(p->h_buf);
     p->h_buf = nullptr;
     p->h_cap = 0;
-    PK_CUDA(cudaMallocHost(&p->h_buf, total * sizeof(int)));
-    p->h_cap = total;
+    PK_CUDA(cudaMallocHost(&p->h_buf, n * sizeof(PackedItem)));
+    p->h_cap = n;
   }
-  if (p->d_cap < total) {
+  if (p->d_cap < n) {
     PK_CUDA(cudaDeviceSynchronize());
     cudaFree(p->d_buf);
     p->d_buf = nullptr;
     p->d_cap = 0;
-    const size_t cap = std::max<size_t>(total, 1024);
-    PK_CUDA(cudaMalloc(&p->d_buf, cap * sizeof(int)));
+    const size_t cap = std::max<size_t>(n, 256);
+    PK_CUDA(cudaMalloc(&p->d_buf, cap * sizeof(PackedItem)));
     p->d_cap = cap;
   }
-  std::memcpy(p->h_buf, docs.data(), ndocs * sizeof(PackedDoc));
-  std::memcpy(p->h_buf + o_row, row.data(), (ndocs + 1) * sizeof(int));
-  PK_CUDA(cudaMemcpyAsync(p->d_buf, p->h_buf, total * sizeof(int), cudaMemcpyHostToDevice, st));
+  for (size_t i = 0; i < n; ++i) p->h_buf[i] = items[i].second;
+  if (n)
+    PK_CUDA(cudaMemcpyAsync(p->d_buf, p->h_buf, n * sizeof(PackedItem), cudaMemcpyHostToDevice, st));
   PK_CUDA(cudaEventRecord(p->uploaded, st));
-  p->o_row = o_row;
-  p->ndocs = ndocs;
   p->nq = nq;
   p->nkv = nkv;
   p->d = d;
   p->window = window;
   p->rows = (int)q0;
   p->keys = (int)k0;
+  p->items = (int)n;
   p->built = true;
   return MOLOT_OK;
 }
 
-template <class T>
-int pk_launch(const molot_packed_plan* p, const PackedArgs& a, cudaStream_t st) {
-  const dim3 grid(p->rows, p->nq);
-  switch (p->d) {
-    case 64: packed_simple_kernel<T, 64><<<grid, 128, 0, st>>>(a); break;
-    case 128: packed_simple_kernel<T, 128><<<grid, 128, 0, st>>>(a); break;
-    default: packed_simple_kernel<T, 256><<<grid, 128, 0, st>>>(a); break;
-  }
+// [rows][heads][d] with `stride` elements between rows, read in boxes of 64
+// elements x `bh` heads x `br` rows.
+int pk_map(CUtensorMap* map, const void* base, bool bf, int d, int heads, int rows,
+           long long stride, int bh, int br) {
+  static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault,
+                                         &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      fn = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  }();
+  if (!encode) return pk_fail(MOLOT_ERR_CUDA, "cuTensorMapEncodeTiled not available");
+  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)stride * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)bh, (cuuint32_t)br}, es[3] = {1, 1, 1};
+  const CUresult r =
+      encode(map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+             const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return pk_fail(MOLOT_ERR_CUDA, "cuTensorMapEncodeTiled");
+  return MOLOT_OK;
+}
+
+struct PkMaps {
+  CUtensorMap q, k, v;
+};
+
+template <class T, int D, int M>
+int pk_run(const molot_packed_plan* p, const PkMaps& m, const PackedArgs& a, cudaStream_t st) {
+  using S = PackedShape<D>;
+  PK_CUDA(cudaFuncSetAttribute(packed_kernel<T, D, M>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               S::kSmem));
+  packed_kernel<T, D, M><<<p->items * p->nkv, S::kThreads, S::kSmem, st>>>(m.q, m.k, m.v, a);
   return pk_cuda(cudaGetLastError(), "packed attention launch");
+}
+
+template <class T, int D>
+int pk_mode(const molot_packed_plan* p, const PkMaps& m, const PackedArgs& a, cudaStream_t st) {
+  if (a.cap > 0.f) return pk_run<T, D, kCap>(p, m, a, st);
+  // kPlain takes maxima before the scale
+  if (a.slopes || a.scale < 0.f) return pk_run<T, D, kBias>(p, m, a, st);
+  return pk_run<T, D, kPlain>(p, m, a, st);
+}
+
+template <class T>
+int pk_launch(const molot_packed_plan* p, const PkMaps& m, const PackedArgs& a, cudaStream_t st) {
+  switch (p->d) {
+    case 64: return pk_mode<T, 64>(p, m, a, st);
+    case 128: return pk_mode<T, 128>(p, m, a, st);
+    default: return pk_mode<T, 256>(p, m, a, st);
+  }
 }
 
 }  // namespace
@@ -129,6 +193,14 @@ int molot_packed_plan_create(molot_packed_plan** out) {
     delete p;
     return rc;
   }
+  cudaError_t e = cudaMalloc(&p->status, 256);
+  if (e == cudaSuccess) e = cudaMemset(p->status, 0, 256);
+  if (e != cudaSuccess) {
+    cudaFree(p->status);
+    cudaEventDestroy(p->uploaded);
+    delete p;
+    return pk_cuda(e, "cudaMalloc(status)");
+  }
   *out = p;
   return MOLOT_OK;
 }
@@ -141,6 +213,7 @@ void molot_packed_plan_destroy(molot_packed_plan* p) {
   cudaDeviceSynchronize();
   cudaFreeHost(p->h_buf);
   cudaFree(p->d_buf);
+  cudaFree(p->status);
   cudaEventDestroy(p->uploaded);
   if (prev >= 0) cudaSetDevice(prev);
   delete p;
@@ -154,6 +227,7 @@ int molot_packed_plan_build(molot_packed_plan* p, int ndocs, int nq, int nkv, in
     return pk_fail(MOLOT_ERR_INVALID, "nq must be a multiple of nkv");
   if (d != 64 && d != 128 && d != 256)
     return pk_fail(MOLOT_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256");
+  if (nq / nkv > 128) return pk_fail(MOLOT_ERR_UNSUPPORTED, "nq / nkv must be at most 128");
   int dev = -1;
   PK_CUDA(cudaGetDevice(&dev));
   if (dev != p->device) return pk_fail(MOLOT_ERR_INVALID, "plan used on another device");
@@ -188,11 +262,31 @@ int molot_packed_attend(molot_packed_plan* p, const void* q, const void* k, cons
   int dev = -1;
   PK_CUDA(cudaGetDevice(&dev));
   if (dev != p->device) return pk_fail(MOLOT_ERR_INVALID, "plan used on another device");
-  const PackedArgs a{q, k, v, o, lse, slopes, reinterpret_cast<const PackedDoc*>(p->d_buf),
-                     p->d_buf + p->o_row, q_stride, k_stride, v_stride, p->ndocs, p->nq,
-                     p->nq / p->nkv, p->window, scale, softcap};
-  return act_dtype == MOLOT_ACT_BF16 ? pk_launch<__nv_bfloat16>(p, a, (cudaStream_t)stream)
-                                     : pk_launch<__half>(p, a, (cudaStream_t)stream);
+  const int G = p->nq / p->nkv, bp = 128 / G;
+  const bool bf = act_dtype == MOLOT_ACT_BF16;
+  PkMaps m;
+  // without keys nothing is read through the K and V maps
+  const void* kb = p->keys ? k : q;
+  const void* vb = p->keys ? v : q;
+  const int keys = std::max(p->keys, 1);
+  if (int rc = pk_map(&m.q, q, bf, p->d, p->nq, p->rows, q_stride, G, bp)) return rc;
+  if (int rc = pk_map(&m.k, kb, bf, p->d, p->nkv, keys, k_stride, 1, pk_bn(p->d))) return rc;
+  if (int rc = pk_map(&m.v, vb, bf, p->d, p->nkv, keys, v_stride, 1, pk_bn(p->d))) return rc;
+  const PackedArgs a{o, lse, slopes, p->d_buf, p->status, p->nq, p->nkv, G, bp, p->window,
+                     scale, softcap, kPkWaitNs};
+  return bf ? pk_launch<__nv_bfloat16>(p, m, a, (cudaStream_t)stream)
+            : pk_launch<__half>(p, m, a, (cudaStream_t)stream);
+}
+
+int molot_packed_check(molot_packed_plan* p, void* stream) {
+  if (!p) return pk_fail(MOLOT_ERR_INVALID, "null plan");
+  int code = 0;
+  PK_CUDA(cudaMemcpyAsync(&code, p->status, sizeof code, cudaMemcpyDeviceToHost,
+                          (cudaStream_t)stream));
+  PK_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+  if (!code) return MOLOT_OK;
+  PK_CUDA(cudaMemsetAsync(p->status, 0, sizeof code, (cudaStream_t)stream));
+  return pk_fail(MOLOT_ERR_TIMEOUT, "a packed attention launch gave up on a bounded wait");
 }
 
 }  // extern "C"
