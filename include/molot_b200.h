@@ -487,6 +487,9 @@ int molot_f8b_write(molot_f8b_plan* plan, const molot_f8b_layer* layer, const vo
 int molot_f8b_decode(molot_f8b_plan* plan, const molot_f8b_layer* layer, const void* q, void* o,
                      float* lse, int act_dtype, long long q_stride, float scale, float softcap,
                      const float* slopes, float* weight_out, void* stream);
+/* Synchronises `stream` and reports (then clears) a decode of the plan that
+ * gave up on a bounded wait: MOLOT_ERR_TIMEOUT, its outputs are garbage. */
+int molot_f8b_check(molot_f8b_plan* plan, void* stream);
 /* Per sequence and kv head, keeps `budget` of the plan's seq_len slots: the
  * newest `recent`, and of the others those with the largest counters (equal
  * ones: the lowest slot first; NaN last).  Their rows move, in order, to

@@ -177,6 +177,7 @@ _decl("molot_f8b_plan_destroy", [_p], None)
 _decl("molot_f8b_plan_build", [_p, _i, _i, _i, _i, _p, _p, _p, _p, _i, _p])
 _decl("molot_f8b_write", [_p, _lp, _p, _p, _i, _ll, _ll, _p])
 _decl("molot_f8b_decode", [_p, _lp, _p, _p, _p, _i, _ll, _f, _f, _p, _p, _p])
+_decl("molot_f8b_check", [_p, _p])
 _decl("molot_f8b_evict", [_p, _lp, _lp, _i, _i, _p, _p])
 _decl("molot_packed_plan_create", [_pp])
 _decl("molot_packed_plan_destroy", [_p], None)
@@ -777,6 +778,9 @@ class F8Plan:
             None if weight_out is None else _cuda_f32(weight_out, "weight_out",
                                                       layer.weight_shape),
             _stream_ptr(stream)))
+
+    def check(self, stream=None) -> None:
+        check(_lib.molot_f8b_check(self._h, _stream_ptr(stream)))
 
     def evict(self, src, dst, budget, recent, kept, stream=None) -> None:
         """Moves the slots to keep from src to dst (pages of its own);

@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "molot_b200.h"
+#include "tensor_map.cuh"
 
 namespace molot {
 int set_last_error(int code, const char* msg);
@@ -75,6 +76,7 @@ struct molot_f8b_plan {
   size_t rec_cap = 0;    // floats
   int* tickets = nullptr;
   size_t tickets_cap = 0;
+  int* status = nullptr;
   int sms = 0;
   bool has_empty = false;
 
@@ -199,6 +201,23 @@ int f8_build(molot_f8b_plan* p, int B, int nq, int nkv, int d, const int* seq_le
   return MOLOT_OK;
 }
 
+// Rows of d bytes of a code pool, read in boxes of 16 rows (a block) x 128
+// bytes at most.  The pool's length is the caller's to keep: the map's rows
+// only bound what a wrong block table could reach.
+int f8_map(CUtensorMap* map, const void* base, int d) {
+  const auto encode = tensor_map_encoder();
+  if (!encode) return f8_fail(MOLOT_ERR_CUDA, "cuTensorMapEncodeTiled not available");
+  const cuuint64_t dims[2] = {(cuuint64_t)d, 0x7ffffff0ull}, strides[1] = {(cuuint64_t)d};
+  const cuuint32_t box[2] = {(cuuint32_t)std::min(d, 128), kF8Blk}, es[2] = {1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
+                            strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            d == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MOLOT_OK : f8_fail(MOLOT_ERR_CUDA, "cuTensorMapEncodeTiled");
+}
+
+constexpr unsigned long long kF8WaitNs = 2000000000ull;  // 2 s per bounded wait
+
 // Checks a layer's pools for slots [0, max_len) of every sequence.
 int f8_pool(const molot_f8b_plan* p, const molot_f8b_layer* l, int max_len, F8Pool* out) {
   if (!p || !p->built) return f8_fail(MOLOT_ERR_INVALID, "plan not built");
@@ -240,6 +259,14 @@ int molot_f8b_plan_create(molot_f8b_plan** out) {
     delete p;
     return rc;
   }
+  cudaError_t e = cudaMalloc(&p->status, 256);
+  if (e == cudaSuccess) e = cudaMemset(p->status, 0, 256);
+  if (e != cudaSuccess) {
+    cudaFree(p->status);
+    cudaEventDestroy(p->uploaded);
+    delete p;
+    return f8_cuda(e, "cudaMalloc(status)");
+  }
   *out = p;
   return MOLOT_OK;
 }
@@ -255,6 +282,7 @@ void molot_f8b_plan_destroy(molot_f8b_plan* p) {
   cudaFree(p->score);
   cudaFree(p->rec);
   cudaFree(p->tickets);
+  cudaFree(p->status);
   cudaEventDestroy(p->uploaded);
   if (prev >= 0) cudaSetDevice(prev);
   delete p;
@@ -350,8 +378,13 @@ int molot_f8b_decode(molot_f8b_plan* p, const molot_f8b_layer* layer, const void
   a.HG = (G + 7) / 8;
   a.items = p->visits * a.HG;
   a.has_empty = p->has_empty;
+  a.status = p->status;
+  a.timeout_ns = kF8WaitNs;
   a.scale = scale;
   a.cap = softcap;
+  CUtensorMap mk, mv;
+  if (int rc = f8_map(&mk, layer->k, p->d)) return rc;
+  if (int rc = f8_map(&mv, layer->v, p->d)) return rc;
   if (int rc = f8_dispatch(act_dtype, p->d, [&](auto t, auto dd) {
         using F = F8Dec<decltype(t), decltype(dd)::value>;
         const auto kernel = f8_decode_kernel<decltype(t), decltype(dd)::value>;
@@ -361,7 +394,7 @@ int molot_f8b_decode(molot_f8b_plan* p, const molot_f8b_layer* layer, const void
         static_assert(F::kCtas <= kF8MaxCtas, "records");
         const int grid = (int)std::max<long long>(
             1, std::min<long long>(a.items, (long long)F::kCtas * p->sms));
-        kernel<<<grid, kF8Warps * 32, F::kSmem, (cudaStream_t)stream>>>(a);
+        kernel<<<grid, kF8Warps * 32, F::kSmem, (cudaStream_t)stream>>>(mk, mv, a);
         return f8_cuda(cudaGetLastError(), "f8 decode launch");
       }))
     return rc;
@@ -398,6 +431,17 @@ int molot_f8b_evict(molot_f8b_plan* p, const molot_f8b_layer* src, const molot_f
     default: f8_move_kernel<256><<<grid, 128, 0, (cudaStream_t)stream>>>(a); break;
   }
   return f8_cuda(cudaGetLastError(), "f8 move launch");
+}
+
+int molot_f8b_check(molot_f8b_plan* p, void* stream) {
+  if (!p) return f8_fail(MOLOT_ERR_INVALID, "null plan");
+  int code = 0;
+  F8_CUDA(cudaMemcpyAsync(&code, p->status, sizeof code, cudaMemcpyDeviceToHost,
+                          (cudaStream_t)stream));
+  F8_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+  if (!code) return MOLOT_OK;
+  F8_CUDA(cudaMemsetAsync(p->status, 0, sizeof code, (cudaStream_t)stream));
+  return f8_fail(MOLOT_ERR_TIMEOUT, "a decode launch gave up on a bounded wait");
 }
 
 }  // extern "C"

@@ -15,6 +15,7 @@
 // costs no accuracy against amax / 448.  Infinities saturate, NaN stays NaN.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
@@ -181,7 +182,8 @@ __global__ void __launch_bounds__(128) f8_write_kernel(const __grid_constant__ F
 // (22 bits); for 16-bit types the query is exact in one part, and one FP16
 // part of the weights is 4 bits finer than BF16.  The dims of a K row and
 // the slots and dims of V are numbered so that a lane's 16-byte loads are
-// its matrix operands: nothing passes through shared memory.
+// its matrix operands.  Blocks come by TMA into a ring of the warp's own in
+// shared memory, swizzled so that those loads touch every bank once.
 //
 // Softmax in base 2 with one reference M per head, raised only when a
 // score passes it by 2^8.  What must not overflow FP16 is the weight times
@@ -189,8 +191,9 @@ __global__ void __launch_bounds__(128) f8_write_kernel(const __grid_constant__ F
 // <= 2^14 multiplies the codes, while l adds 2^(s - M + 38), which stays
 // within FP32 for every ev in [-64, 120].  O = sum(P * code) * 2^32 / l.
 //
-// Bound by the bytes of the cache: a warp keeps one block of K and of V in
-// flight (4 KB at d = 128), 16 warps an SM.
+// Bound by the bytes of the cache, so by what is in flight: with one block
+// of a warp under way in registers (64 KB an SM) the 2.35 M slots x 8 heads
+// of d = 128 took 993 us, nothing else above 45 % busy.
 struct F8DecodeArgs {
   F8Pool pool;
   const F8Seq* seqs;
@@ -207,6 +210,8 @@ struct F8DecodeArgs {
   long long items;
   int B, nq, G, HG;  // HG head groups of up to 8 per kv head
   int has_empty;     // some sequence sees nothing
+  int* status;       // 1 after a bounded wait ran out
+  unsigned long long timeout_ns;
   float scale, cap;
 };
 
@@ -215,29 +220,44 @@ constexpr int kF8Warps = 8;
 template <class T, int D>
 struct F8Dec {
   static constexpr bool kSplit = std::is_same<T, float>::value;
-  static constexpr int KS = D / 16;            // k steps of S, and m tiles of O
-  static constexpr int CH = D / 64;            // 16-byte chunks of a K row per lane
-  static constexpr int VB = D >= 128 ? 16 : 8;  // bytes of a V row's chunk per lane
-  static constexpr int VC = D / 8 / VB;        // chunks
+  static constexpr int KS = D / 16;              // k steps of S, and m tiles of O
+  static constexpr int NH = D == 256 ? 2 : 1;    // halves of a row, 128 bytes at most
+  static constexpr int HB = D / NH;              // bytes of one
+  static constexpr int LW = HB / 16;             // words of a K row's half per lane
+  static constexpr int VB = D >= 128 ? 16 : 8;   // bytes of a V row's half per lane
   static constexpr int kCtas = D == 256 ? 1 : 2;
-  static constexpr int kFrag = KS * 32 * 4;      // floats of O in fragment order
-  static constexpr int kRec = kFrag + 16;        // + M[8], l[8]
-  static constexpr int kQ = KS * 32 * 8;         // bytes of one FP16 part of Q
-  static constexpr int kSmem = kF8Warps * kRec * 4 + 2 * kQ + 64;
+  // Ring of blocks per warp: 192 KB an SM in flight
+  static constexpr int kStages = D == 64 ? 6 : 3;
+  static constexpr int kBlk = 2 * kF8Blk * D;  // bytes of K and V of a block
+  static constexpr int kRing = kF8Warps * kStages * kBlk;
+  static constexpr int kFrag = KS * 32 * 4;  // floats of O in fragment order
+  static constexpr int kRec = kFrag + 16;    // + M[8], l[8]
+  static constexpr int kQ = KS * 32 * 8;     // bytes of one FP16 part of Q
+  static constexpr int kBar = kRing + 2 * kQ + 64;
+  static constexpr int kSmem = kBar + kF8Warps * kStages * 8 + 1024;  // + alignment
+  static_assert(kRing >= kF8Warps * kRec * 4, "the warps' records take the ring's place");
 };
 
-__device__ __forceinline__ uint4 ldg_stream(const void* p) {
+// TMA: box of 16 rows at byte x (0 or 128) and row y of a pool.
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                         uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(ptx::smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
+               : "r"(a)
+               : "memory");
   return v;
 }
-__device__ __forceinline__ uint2 ldg_stream2(const void* p) {
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
   uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];"
-               : "=r"(v.x), "=r"(v.y)
-               : "l"(p));
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ void cvt4(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -271,19 +291,36 @@ __device__ __forceinline__ uint32_t pack_h2_rest(uint32_t hi, float x, float y) 
 
 template <class T, int D>
 __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
-    f8_decode_kernel(const __grid_constant__ F8DecodeArgs a) {
+    f8_decode_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                     const __grid_constant__ F8DecodeArgs a) {
   using F = F8Dec<T, D>;
-  constexpr int KS = F::KS, CH = F::CH, VC = F::VC;
-  extern __shared__ __align__(16) unsigned char smem[];
-  float* recs = reinterpret_cast<float*>(smem);                     // [warps][kRec]
-  unsigned char* qs = smem + kF8Warps * F::kRec * 4;                // high part, then low
-  float* qinv = reinterpret_cast<float*>(qs + 2 * F::kQ);           // [8]
+  constexpr int KS = F::KS, NH = F::NH;
+  constexpr int kThreads = kF8Warps * 32;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
+  float* recs = reinterpret_cast<float*>(smem);  // [warps][kRec], after the ring
+  unsigned char* qs = smem + F::kRing;           // high part, then low
+  float* qinv = reinterpret_cast<float*>(qs + 2 * F::kQ);  // [8]
   __shared__ int s_last;
+  __shared__ volatile int s_abort;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;  // fragment row group, column pair
   const int nkv = a.pool.nkv, ps = a.pool.page_size, bpp = ps / kF8Blk;
   const long long grid = gridDim.x;
   const long long x0 = blockIdx.x * a.items / grid, x1 = (blockIdx.x + 1) * a.items / grid;
+  const uint32_t ring = ptx::smem_u32(smem) + warp * F::kStages * F::kBlk;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + F::kBar) + warp * F::kStages;
+  // Where this lane's pieces lie in a box: rows of HB bytes, the 16-byte
+  // pieces of row r in the order that the 128-byte (64-byte) swizzle gives.
+  auto piece = [&](int r, int c) {
+    return r * F::HB + ((c ^ (F::HB == 128 ? r & 7 : (r >> 1) & 3)) * 16);
+  };
+  int count = 0, put = 0;  // blocks this warp has waited for, and asked for
+  if (lane == 0)
+    for (int i = 0; i < F::kStages; ++i) ptx::mbar_init(full + i, 1);
+  if (tid == 0) s_abort = 0;
+  ptx::fence_mbar_init();
+  __syncthreads();
 
   for (long long x = x0; x < x1;) {
     // the item's segment
@@ -296,7 +333,46 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
     const int h = seg / a.HG, hg = seg % a.HG;
     const int head0 = h * a.G + hg * 8, nh = min(8, a.G - hg * 8);
     const int* bt = a.pool.bt + (long long)b * a.pool.max_pages;
+    const bool first_piece = x == x0;
     x += i1 - i0;
+
+    // The warp's blocks are i0 + warp + 8 m, m in [0, nm).  They are fetched
+    // kStages ahead; of a run of 32, lane l has block l's place and scales.
+    const int nm = i1 - i0 > warp ? (i1 - i0 - warp + kF8Warps - 1) / kF8Warps : 0;
+    auto block_of = [&](int m) {
+      const int i = i0 + warp + kF8Warps * m;
+      return i < sq.na ? sq.a0 + i : sq.b0 + i - sq.na;
+    };
+    // block index within the pool; K and V of 180 GB hold fewer than 2^31
+    auto place_of = [&](int m) {
+      const int blk = m < nm ? block_of(m) : 0;
+      return m < nm ? (int)(((long long)bt[blk / bpp] * nkv + h) * bpp + blk % bpp) : 0;
+    };
+    int place = place_of(lane), place_next = nm > 32 ? place_of(lane + 32) : 0;
+    float ks_in = 0.f, vs_in = 0.f, ks_run = 0.f, vs_run = 0.f;
+    auto fetch = [&](int m) {
+      if ((m & 31) == 0) {
+        if (m) place = place_next, place_next = place_of(m + 32 + lane);
+        if (m + lane < nm) {
+          ks_in = __ldg(a.pool.k_scale + place);
+          vs_in = __ldg(a.pool.v_scale + place);
+        }
+      }
+      if (lane == (m & 31)) {
+        const int st = put % F::kStages;
+        const uint32_t dst = ring + st * F::kBlk;
+        ptx::mbar_arrive_expect_tx(full + st, F::kBlk);
+#pragma unroll
+        for (int i = 0; i < NH; ++i) {
+          tma_rows(dst + i * kF8Blk * 128, &mk, i * 128, place * kF8Blk, full + st);
+          tma_rows(dst + kF8Blk * D + i * kF8Blk * 128, &mv, i * 128, place * kF8Blk, full + st);
+        }
+      }
+      ++put;
+    };
+#pragma unroll
+    for (int m = 0; m < F::kStages; ++m)
+      if (m < nm) fetch(m);
 
     // Q in operand order, a warp per head
     {
@@ -316,7 +392,10 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         const int dd = lane + 32 * i;
-        const int j = (dd >> 6) * 4 + ((dd & 15) >> 2), tt = (dd & 63) >> 4, r = dd & 3;
+        // lane tt of a row group has the 4 LW bytes of the row's half from
+        // 4 LW tt on, word by word
+        const int hd = dd % F::HB;
+        const int j = dd / F::HB * F::LW + hd / 4 % F::LW, tt = hd / (4 * F::LW), r = dd & 3;
         const int at = (j * 32 + warp * 4 + tt) * 4 + r;
         const __half hi = __float2half_rn(v[i] * up);
         reinterpret_cast<__half*>(qs)[at] = hi;
@@ -341,106 +420,69 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
 #pragma unroll
     for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
-    auto block_of = [&](int i) { return i < sq.na ? sq.a0 + i : sq.b0 + i - sq.na; };
-    uint4 ka[CH], kb[CH];
-    uint4 vr[4][VC];  // slots 2t, 2t + 1, 2t + 8, 2t + 9 (VB = 8: the low halves)
-    float ks = 0.f, vs = 0.f;
-    long long nrow = 0;  // row index (times d: byte offset) of the block being fetched
-    int pages = 0;       // lane l: page of block i + 8 l of the current run
-    auto locate = [&](int i) {  // of block i, page from the run's lane
-      const int k = ((i - i0) / kF8Warps) & 31;
-      if (k == 0) {
-        const int bi = i + lane * kF8Warps;
-        pages = bi < i1 ? bt[block_of(bi) / bpp] : 0;
+    for (int m = 0; m < nm; ++m) {
+      if ((m & 31) == 0) ks_run = ks_in, vs_run = vs_in;
+      const float ksc = __shfl_sync(0xffffffffu, ks_run, m & 31);
+      const float vsc = __shfl_sync(0xffffffffu, vs_run, m & 31);
+      const int st = count % F::kStages;
+      const uint32_t src = ring + st * F::kBlk, vsrc = src + kF8Blk * D;
+      if (!s_abort && !ptx::mbar_wait_bounded(full + st, (count / F::kStages) & 1, a.timeout_ns)) {
+        s_abort = 1;
+        atomicCAS(a.status, 0, 1);
       }
-      const long long page = __shfl_sync(0xffffffffu, pages, k);
-      return ((page * nkv + h) * bpp + block_of(i) % bpp);
-    };
-    auto load_k = [&](long long blk) {
-      ks = __ldg(a.pool.k_scale + blk);
-      const uint8_t* p = a.pool.k + blk * (kF8Blk * D) + g * D + t4 * 16;
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        ka[c] = ldg_stream(p + c * 64);
-        kb[c] = ldg_stream(p + 8 * D + c * 64);
-      }
-    };
-    auto load_v = [&](long long blk) {
-      vs = __ldg(a.pool.v_scale + blk);
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int c = 0; c < VC; ++c) {
-          const uint8_t* p = a.pool.v + blk * (kF8Blk * D) +
-                             (2 * t4 + (r & 1) + (r & 2) * 4) * D + c * 128 + g * F::VB;
-          if (F::VB == 16) {
-            vr[r][c] = ldg_stream(p);
-          } else {
-            const uint2 w = ldg_stream2(p);
-            vr[r][c] = make_uint4(w.x, w.y, 0, 0);
-          }
-        }
-    };
-    int i = i0 + warp;
-    if (i < i1) {
-      nrow = locate(i);
-      load_k(nrow);
-      load_v(nrow);
-    }
-    for (; i < i1; i += kF8Warps) {
+      __syncwarp();
+      ++count;
       // S^T: two chains, so that a product need not wait for the last one
       float s[2][4] = {};
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const uint32_t wa[4] = {ka[c].x, ka[c].y, ka[c].z, ka[c].w};
-        const uint32_t wb[4] = {kb[c].x, kb[c].y, kb[c].z, kb[c].w};
+      for (int c = 0; c < NH; ++c) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int j = c * 4 + w;
-          uint32_t a0, a1, a2, a3;
-          cvt4(wa[w], a0, a2);
-          cvt4(wb[w], a1, a3);
-          mma16816(s[w & 1], a0, a1, a2, a3, qh[j].x, qh[j].y);
-          if (F::kSplit) {
-            const uint2 ql = reinterpret_cast<const uint2*>(qs + F::kQ)[j * 32 + lane];
-            mma16816(s[(w & 1) ^ 1], a0, a1, a2, a3, ql.x, ql.y);
+        for (int e = 0; e < F::LW / 4; ++e) {
+          const uint32_t kp = src + c * kF8Blk * 128;
+          const uint4 ka = lds16(kp + piece(g, t4 * (F::LW / 4) + e));
+          const uint4 kb = lds16(kp + piece(g + 8, t4 * (F::LW / 4) + e));
+          const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int j = c * F::LW + e * 4 + w;
+            uint32_t a0, a1, a2, a3;
+            cvt4(wa[w], a0, a2);
+            cvt4(wb[w], a1, a3);
+            mma16816(s[w & 1], a0, a1, a2, a3, qh[j].x, qh[j].y);
+            if (F::kSplit) {
+              const uint2 ql = reinterpret_cast<const uint2*>(qs + F::kQ)[j * 32 + lane];
+              mma16816(s[(w & 1) ^ 1], a0, a1, a2, a3, ql.x, ql.y);
+            }
           }
         }
       }
-      const float ksc = ks, vsc = vs;
-      const int blk_t = block_of(i) * kF8Blk;
-      const bool more = i + kF8Warps < i1;
-      if (more) {
-        nrow = locate(i + kF8Warps);
-        load_k(nrow);
-      }
+      const int blk_t = block_of(m) * kF8Blk;
       // base-2 scores: [0..1] slot g, [2..3] slot g + 8; heads 2t, 2t + 1
       float z[4];
       {
         const float c0 = ksc * sc0, c1 = ksc * sc1;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float dist = (float)(sq.n - 1 - (blk_t + g + (r >> 1) * 8));
-          z[r] = score_logit((s[0][r] + s[1][r]) * (r & 1 ? c1 : c0), a.cap,
-                             r & 1 ? slope1 : slope0, dist);
+        for (int r = 0; r < 4; ++r) z[r] = (s[0][r] + s[1][r]) * (r & 1 ? c1 : c0);
+        if (a.cap > 0.f) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) z[r] = a.cap * tanhf(z[r] / a.cap);
         }
+        const float dist = (float)(sq.n - 1 - (blk_t + g));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          z[r] = (z[r] - (r & 1 ? slope1 : slope0) * (dist - (r >> 1) * 8)) * kLog2e;
       }
       const bool edge = blk_t < sq.first || blk_t + kF8Blk > sq.n ||
                         (blk_t < sq.lo && blk_t + kF8Blk > sq.sink_end);
-      if (edge) {  // mask slots, and zero V where a code may be NaN
-        auto see = [&](int t) {
-          return t >= sq.first && t < sq.n && (t >= sq.lo || t < sq.sink_end);
-        };
+      auto see = [&](int t) {
+        return t >= sq.first && t < sq.n && (t >= sq.lo || t < sq.sink_end);
+      };
+      if (edge) {
         if (!see(blk_t + g)) z[0] = z[1] = -CUDART_INF_F;
         if (!see(blk_t + g + 8)) z[2] = z[3] = -CUDART_INF_F;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (!see(blk_t + 2 * t4 + (r & 1) + (r & 2) * 4)) {
-#pragma unroll
-            for (int c = 0; c < VC; ++c) vr[r][c] = make_uint4(0, 0, 0, 0);
-          }
       }
       if (a.score) {
+        const int i = i0 + warp + kF8Warps * m;
         float* sp = a.score + (((long long)a.prefix[b] + (long long)h * sq.nblk + i) * kF8Blk + g) *
                                   a.G + hg * 8 + 2 * t4;
         if (2 * t4 < nh) sp[0] = z[0], sp[8 * a.G] = z[2];
@@ -466,12 +508,14 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
           o[k][1] *= f1, o[k][3] *= f1;
         }
       }
-      const float r0 = 38.f - m0, r1 = 38.f - m1;
+      // (no score yet: -inf + 0, a weight of 0)
+      const float r0 = m0 == -CUDART_INF_F ? 0.f : 38.f - m0;
+      const float r1 = m1 == -CUDART_INF_F ? 0.f : 38.f - m1;
       const float up = vsc * 0x1p-32f;  // 2^(ev - 32)
       float p[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        p[r] = z[r] == -CUDART_INF_F ? 0.f : ex2(z[r] + (r & 1 ? r1 : r0));
+        p[r] = ex2(z[r] + (r & 1 ? r1 : r0));
       l0 += p[0] + p[2];
       l1 += p[1] + p[3];
 #pragma unroll
@@ -484,26 +528,41 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
         e1 = movmatrix_trans(pack_h2_rest(h1, p[2], p[3]));
       }
 #pragma unroll
-      for (int c = 0; c < VC; ++c) {
+      for (int c = 0; c < NH; ++c) {
+        uint4 vr[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 2 * t4 + (r & 1) + (r & 2) * 4;
+          const uint32_t vp = vsrc + c * kF8Blk * 128;
+          if (F::VB == 16) {
+            vr[r] = lds16(vp + piece(row, g));
+          } else {
+            const uint2 w = lds8(vp + piece(row, g >> 1) + (g & 1) * 8);
+            vr[r] = make_uint4(w.x, w.y, 0, 0);
+          }
+          // a masked slot's codes may be NaN, and 0 * NaN is NaN
+          if (edge && !see(blk_t + row)) vr[r] = make_uint4(0, 0, 0, 0);
+        }
+        const uint32_t* v0 = &vr[0].x;
+        const uint32_t* v1 = &vr[1].x;
+        const uint32_t* v2 = &vr[2].x;
+        const uint32_t* v3 = &vr[3].x;
 #pragma unroll
         for (int w = 0; w < F::VB / 4; ++w) {
-          const uint32_t* x0w = &vr[0][c].x;
-          const uint32_t* x1w = &vr[1][c].x;
-          const uint32_t* x2w = &vr[2][c].x;
-          const uint32_t* x3w = &vr[3][c].x;
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const uint32_t sel = u ? 0x7362 : 0x5140;
             uint32_t a0, a1, a2, a3;
-            cvt4(__byte_perm(x0w[w], x1w[w], sel), a0, a1);
-            cvt4(__byte_perm(x2w[w], x3w[w], sel), a2, a3);
+            cvt4(__byte_perm(v0[w], v1[w], sel), a0, a1);
+            cvt4(__byte_perm(v2[w], v3[w], sel), a2, a3);
             const int k = c * (F::VB / 2) + 2 * w + u;
             mma16816(o[k], a0, a1, a2, a3, b0, b1);
             if (F::kSplit) mma16816(o[k], a0, a1, a2, a3, e0, e1);
           }
         }
       }
-      if (more) load_v(nrow);
+      __syncwarp();  // every lane has read the stage
+      if (m + F::kStages < nm) fetch(m + F::kStages);
     }
 
     // merge the warps: records in fragment order, then one sum per position
@@ -512,6 +571,7 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
       l0 += __shfl_xor_sync(0xffffffffu, l0, k);
       l1 += __shfl_xor_sync(0xffffffffu, l1, k);
     }
+    __syncthreads();  // every warp is done with the ring
     {
       float* r = recs + warp * F::kRec;
 #pragma unroll
@@ -524,31 +584,11 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
     }
     __syncthreads();
 
-    // Sums of n records (stride st floats) at fragment position f4 for heads
-    // 2t, 2t + 1; M and l of the heads along with it.
-    auto gather = [&](const float* r, int n, long long st, int f4, float4& acc, float2& mm,
-                      float2& ll) {
-      const int hh = 2 * (f4 & 3);
-      mm = make_float2(-CUDART_INF_F, -CUDART_INF_F);
-#pragma unroll 8
-      for (int k = 0; k < n; ++k) {
-        const float2 v = *reinterpret_cast<const float2*>(r + k * st + F::kFrag + hh);
-        mm.x = fmaxf(mm.x, v.x), mm.y = fmaxf(mm.y, v.y);
-      }
-      acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      ll = make_float2(0.f, 0.f);
-#pragma unroll 8
-      for (int k = 0; k < n; ++k) {
-        const float* rk = r + k * st;
-        const float2 mv = *reinterpret_cast<const float2*>(rk + F::kFrag + hh);
-        const float2 lv = *reinterpret_cast<const float2*>(rk + F::kFrag + 8 + hh);
-        const float4 v = reinterpret_cast<const float4*>(rk)[f4];
-        const float fx = mv.x == -CUDART_INF_F ? 0.f : ex2(mv.x - mm.x);
-        const float fy = mv.y == -CUDART_INF_F ? 0.f : ex2(mv.y - mm.y);
-        ll.x += fx * lv.x, ll.y += fy * lv.y;
-        acc.x += fx * v.x, acc.z += fx * v.z;
-        acc.y += fy * v.y, acc.w += fy * v.w;
-      }
+    // Positions of a fragment that hold a head of this group: lanes with
+    // t < th, th 1, 2 or 4.
+    const int th = nh > 4 ? 4 : nh > 2 ? 2 : 1, np = KS * 8 * th;
+    auto position = [&](int i) {
+      return th == 4 ? i : (i / (8 * th)) * 32 + (i / th) % 8 * 4 + i % th;
     };
     // O, log-sum-exp of position f4: dims dim, dim + 1 of heads 2t, 2t + 1
     auto finish = [&](int f4, const float4& acc, const float2& mm, const float2& ll) {
@@ -565,19 +605,35 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
         Act<T>::store(op, (y ? acc.y : acc.x) * inv);
         Act<T>::store(op + 1, (y ? acc.w : acc.z) * inv);
         if (k == 0 && gg == 0) {
-          const float z = l == 0.f ? -CUDART_INF_F : (y ? mm.y : mm.x) - 38.f + log2f(l);
-          if (a.lse) a.lse[row] = z * kLn2;
-          if (a.lse2) a.lse2[row] = z;
+          const float zz = l == 0.f ? -CUDART_INF_F : (y ? mm.y : mm.x) - 38.f + log2f(l);
+          if (a.lse) a.lse[row] = zz * kLn2;
+          if (a.lse2) a.lse2[row] = zz;
         }
       }
     };
     const bool whole = i0 == 0 && i1 == sq.nblk;
-    float* rec = nullptr;
-    if (!whole) rec = a.rec + (2 * (long long)blockIdx.x + (x - (i1 - i0) == x0 ? 0 : 1)) * F::kRec;
-    for (int f4 = tid; f4 < KS * 32; f4 += kF8Warps * 32) {
-      float4 acc;
-      float2 mm, ll;
-      gather(recs, kF8Warps, F::kRec, f4, acc, mm, ll);
+    float* rec = a.rec + (2 * (long long)blockIdx.x + (first_piece ? 0 : 1)) * F::kRec;
+    for (int i = tid; i < np; i += kThreads) {
+      const int f4 = position(i), hh = 2 * (f4 & 3);
+      float2 mm = make_float2(-CUDART_INF_F, -CUDART_INF_F), ll = make_float2(0.f, 0.f);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kF8Warps; ++k) {
+        const float2 v = *reinterpret_cast<const float2*>(recs + k * F::kRec + F::kFrag + hh);
+        mm.x = fmaxf(mm.x, v.x), mm.y = fmaxf(mm.y, v.y);
+      }
+#pragma unroll
+      for (int k = 0; k < kF8Warps; ++k) {
+        const float* rk = recs + k * F::kRec;
+        const float2 mv = *reinterpret_cast<const float2*>(rk + F::kFrag + hh);
+        const float2 lv = *reinterpret_cast<const float2*>(rk + F::kFrag + 8 + hh);
+        const float4 v = reinterpret_cast<const float4*>(rk)[f4];
+        const float fx = mv.x == -CUDART_INF_F ? 0.f : ex2(mv.x - mm.x);
+        const float fy = mv.y == -CUDART_INF_F ? 0.f : ex2(mv.y - mm.y);
+        ll.x += fx * lv.x, ll.y += fy * lv.y;
+        acc.x += fx * v.x, acc.z += fx * v.z;
+        acc.y += fy * v.y, acc.w += fy * v.w;
+      }
       if (whole) {
         finish(f4, acc, mm, ll);
       } else {
@@ -593,46 +649,95 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
       const long long y0 = base + (long long)seg * sq.nblk, y1 = y0 + sq.nblk - 1;
       const long long c0 = ((y0 + 1) * grid + a.items - 1) / a.items - 1;
       const long long c1 = ((y1 + 1) * grid + a.items - 1) / a.items - 1;
+      const int n = (int)(c1 - c0) + 1;
       __threadfence();
       __syncthreads();
       if (tid == 0) {
         int* tk = a.tickets + ((long long)b * nkv + h) * a.HG + hg;
-        const bool last = ptx::atom_add_acq_rel_gpu(tk, 1) == (int)(c1 - c0);
+        const bool last = ptx::atom_add_acq_rel_gpu(tk, 1) == n - 1;
         if (last) *tk = 0;
         s_last = last;
       }
       __syncthreads();
       if (s_last) {
         __threadfence();
-        // the first CTA's record is its first one when the segment starts
-        // its range, else its last; the others' ranges start inside
-        const long long first = 2 * c0 + (c0 * a.items / grid == y0 ? 0 : 1);
-        const int n = (int)(c1 - c0);
-        for (int f4 = tid; f4 < KS * 32; f4 += kF8Warps * 32) {
-          float4 acc, acc1;
-          float2 mm, ll, mm1, ll1;
-          gather(a.rec + first * F::kRec, 1, 0, f4, acc1, mm1, ll1);
-          gather(a.rec + 2 * (c0 + 1) * F::kRec, n, 2 * F::kRec, f4, acc, mm, ll);
-          const float nx = fmaxf(mm.x, mm1.x), ny = fmaxf(mm.y, mm1.y);
-          const float ax = mm1.x == -CUDART_INF_F ? 0.f : ex2(mm1.x - nx);
-          const float ay = mm1.y == -CUDART_INF_F ? 0.f : ex2(mm1.y - ny);
-          const float bx = mm.x == -CUDART_INF_F ? 0.f : ex2(mm.x - nx);
-          const float by = mm.y == -CUDART_INF_F ? 0.f : ex2(mm.y - ny);
-          acc = make_float4(acc1.x * ax + acc.x * bx, acc1.y * ay + acc.y * by,
-                            acc1.z * ax + acc.z * bx, acc1.w * ay + acc.w * by);
-          ll = make_float2(ll1.x * ax + ll.x * bx, ll1.y * ay + ll.y * by);
-          finish(f4, acc, make_float2(nx, ny), ll);
+        // The first CTA's record is its first one when the segment starts
+        // its range, else its last; the others' ranges start inside.
+        const int off0 = c0 * a.items / grid == y0 ? 0 : 1;
+        auto record = [&](int k) { return a.rec + (2 * (c0 + k) + (k ? 0 : off0)) * F::kRec; };
+        // factors of the records: [n][8] M, then l, then the heads' M, l
+        float* fac = reinterpret_cast<float*>(smem);
+        float* fl = fac + n * 8;
+        float* tot = fl + n * 8;  // M[8], l[8]
+        for (int i = tid; i < n * 8; i += kThreads) {
+          fac[i] = record(i >> 3)[F::kFrag + (i & 7)];
+          fl[i] = record(i >> 3)[F::kFrag + 8 + (i & 7)];
+        }
+        __syncthreads();
+        if (warp < nh) {  // a warp per head
+          float mm = -CUDART_INF_F, ll = 0.f;
+          for (int k = lane; k < n; k += 32) mm = fmaxf(mm, fac[k * 8 + warp]);
+          mm = warp_max(mm);
+          for (int k = lane; k < n; k += 32) {
+            const float v = fac[k * 8 + warp];
+            const float f = v == -CUDART_INF_F ? 0.f : ex2(v - mm);
+            fac[k * 8 + warp] = f;
+            ll += f * fl[k * 8 + warp];
+          }
+#pragma unroll
+          for (int k = 16; k; k >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, k);
+          if (lane == 0) tot[warp] = mm, tot[8 + warp] = ll;
+        } else if (lane == 0) {
+          for (int k = 0; k < n; ++k) fac[k * 8 + warp] = 0.f;
+        }
+        __syncthreads();
+        // Threads left over share the records of a position.
+        const int ng = max(1, kThreads / np), grp = tid / np;
+        float4* part = reinterpret_cast<float4*>(tot + 16);
+        for (int i = tid % np + (grp < ng ? 0 : np); i < np; i += kThreads) {
+          const int f4 = position(i), hh = 2 * (f4 & 3);
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+          for (int k = grp; k < n; k += ng) {
+            const float4 v = reinterpret_cast<const float4*>(record(k))[f4];
+            const float2 f = *reinterpret_cast<const float2*>(fac + k * 8 + hh);
+            acc.x += f.x * v.x, acc.z += f.x * v.z;
+            acc.y += f.y * v.y, acc.w += f.y * v.w;
+          }
+          if (ng == 1)
+            finish(f4, acc, *reinterpret_cast<float2*>(tot + hh),
+                   *reinterpret_cast<float2*>(tot + 8 + hh));
+          else
+            part[tid] = acc;
+        }
+        if (ng > 1) {
+          __syncthreads();
+          if (tid < np) {
+            const int f4 = position(tid), hh = 2 * (f4 & 3);
+            float4 acc = part[tid];
+            for (int k = 1; k < ng; ++k) {
+              const float4 v = part[tid + k * np];
+              acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+            }
+            finish(f4, acc, *reinterpret_cast<float2*>(tot + hh),
+                   *reinterpret_cast<float2*>(tot + 8 + hh));
+          }
         }
       }
     }
-    __syncthreads();  // shared memory is free for the next segment
+    // shared memory is free for the next segment's copies
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
   }
+  if (s_abort)  // copies in flight end before the CTA does
+    for (int k = max(0, put - F::kStages); k < put; ++k)
+      ptx::mbar_wait_bounded(full + k % F::kStages, (k / F::kStages) & 1, a.timeout_ns);
   if (a.has_empty)
     for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
       if (a.seqs[b].nblk > 0) continue;
-      for (int i = tid; i < a.nq * D; i += kF8Warps * 32)
+      for (int i = tid; i < a.nq * D; i += kThreads)
         Act<T>::store(static_cast<T*>(a.o) + (long long)b * a.nq * D + i, 0.f);
-      for (int i = tid; i < a.nq; i += kF8Warps * 32) {
+      for (int i = tid; i < a.nq; i += kThreads) {
         if (a.lse) a.lse[(long long)b * a.nq + i] = -CUDART_INF_F;
         if (a.lse2) a.lse2[(long long)b * a.nq + i] = -CUDART_INF_F;
       }

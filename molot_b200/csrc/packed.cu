@@ -1,7 +1,7 @@
 // C ABI of packed-document prefill attention (molot_packed_*).
 #include "packed.cuh"
 
-#include <cudaTypedefs.h>
+#include "tensor_map.cuh"
 
 #include <algorithm>
 #include <cstdio>
@@ -121,15 +121,7 @@ int pk_build(molot_packed_plan* p, int ndocs, const int* q_lens, const int* k_le
 // elements x `bh` heads x `br` rows.
 int pk_map(CUtensorMap* map, const void* base, bool bf, int d, int heads, int rows,
            long long stride, int bh, int br) {
-  static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault,
-                                         &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      fn = nullptr;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-  }();
+  const auto encode = tensor_map_encoder();
   if (!encode) return pk_fail(MOLOT_ERR_CUDA, "cuTensorMapEncodeTiled not available");
   const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)rows};
   const cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)stride * 2};
