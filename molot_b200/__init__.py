@@ -54,6 +54,7 @@ _KV_DTYPES = {"f32": KV_F32, "bf16": KV_BF16, "q8": KV_Q8}
 
 _POOL_DTYPES = dict(_KV_DTYPES, f8b=KV_F8B)
 _ACT_DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}  # molot_act_dtype
+_ACT_CACHE = {}  # the same by dtype object: naming a dtype costs more than the lookup
 
 
 def q8_row_bytes(hd: int) -> int:
@@ -663,27 +664,56 @@ class PagedPlan:
 
 
 def _cuda_f32(t, name, shape=None):
-    _check_cuda_tensor(t, name)
+    if _act_dtype(t) != 0 or not t.is_cuda:
+        raise ValueError(f"{name} must be a float32 CUDA tensor")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must have shape {tuple(shape)}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have shape {shape}")
     return t.data_ptr()
+
+
+def _act_dtype(t):
+    """molot_act_dtype of a tensor, or None."""
+    ty = getattr(t, "dtype", None)
+    act = _ACT_CACHE.get(ty)
+    if act is None:
+        act = _ACT_DTYPES.get(str(ty))
+        if act is not None:
+            _ACT_CACHE[ty] = act
+    return act
 
 
 def _rows(t, name, n, heads, d, act=None):
     """Pointer, row stride and molot_act_dtype of rows [n][heads][d] whose
     heads are contiguous (a part of a wider projection's rows will do)."""
-    if not (hasattr(t, "is_cuda") and t.is_cuda):
-        raise ValueError(f"{name} must be a CUDA tensor")
-    ty = _ACT_DTYPES.get(str(t.dtype))
-    if ty is None or (act is not None and ty != act):
-        raise ValueError(f"{name} must be float32, bfloat16 or float16, like the other operands")
-    if tuple(t.shape) != (n, heads, d):
+    ty = _act_dtype(t)
+    if ty is None or not t.is_cuda or (act is not None and ty != act):
+        raise ValueError(f"{name} must be a float32, bfloat16 or float16 CUDA tensor, "
+                         "like the other operands")
+    if t.shape != (n, heads, d):
         raise ValueError(f"{name} must have shape {(n, heads, d)}")
-    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != d):
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or (heads > 1 and s1 != d):
         raise ValueError(f"{name} must have contiguous heads")
-    return t.data_ptr(), t.stride(0) if n > 1 else heads * d, ty
+    return t.data_ptr(), s0 if n > 1 else heads * d, ty
+
+
+def _current_stream(stream):
+    """Stream pointer for a launch: torch's current stream when None."""
+    if stream is None:
+        global _raw_stream
+        if _raw_stream is None:
+            import torch
+            get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+            device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+            _raw_stream = (lambda: get(device())) if get else \
+                (lambda: torch.cuda.current_stream().cuda_stream)
+        return _raw_stream()
+    return _stream_ptr(stream)
+
+
+_raw_stream = None
 
 
 class F8Layer:
@@ -712,6 +742,8 @@ class F8Layer:
             _cuda_f32(v_scale, "v_scale", sc),
             None if weight is None else _cuda_f32(weight, "weight", self.weight_shape),
             block_table.data_ptr(), self.max_pages, ps)
+        self._ref = ctypes.byref(self._s)
+        self._key = (nkv, d, self.batch)
 
 
 class F8Plan:
@@ -746,21 +778,22 @@ class F8Plan:
         check(_lib.molot_f8b_plan_build(self._h, arrays[0].size, nq, nkv, d,
                                         *(_ptr(a) for a in arrays), window, _stream_ptr(stream)))
         self.B, self.nq, self.nkv, self.d = arrays[0].size, nq, nkv, d
+        self._key = (nkv, d, self.B)
         self.rows = int(np.minimum(arrays[0], 1).sum() if arrays[1] is None else arrays[1].sum())
 
     def _layer(self, layer, name="layer"):
         if not self.B:
             raise ValueError("plan not built")
-        if (layer.nkv, layer.d) != (self.nkv, self.d) or layer.batch != self.B:
+        if layer._key != self._key:
             raise ValueError(f"{name} does not fit the plan's heads or batch")
-        return ctypes.byref(layer._s)
+        return layer._ref
 
     def write(self, layer, k, v, stream=None) -> None:
         """k, v [new rows][nkv][d] float32, bfloat16 or float16."""
         lp = self._layer(layer)
         kp, ks, ty = _rows(k, "k", self.rows, self.nkv, self.d)
         vp, vs, _ = _rows(v, "v", self.rows, self.nkv, self.d, ty)
-        check(_lib.molot_f8b_write(self._h, lp, kp, vp, ty, ks, vs, _stream_ptr(stream)))
+        check(_lib.molot_f8b_write(self._h, lp, kp, vp, ty, ks, vs, _current_stream(stream)))
 
     def decode(self, layer, q, o, scale, softcap=0.0, slopes=None, lse=None, weight_out=None,
                stream=None) -> None:
@@ -777,10 +810,10 @@ class F8Plan:
             None if slopes is None else _cuda_f32(slopes, "slopes", (self.nq,)),
             None if weight_out is None else _cuda_f32(weight_out, "weight_out",
                                                       layer.weight_shape),
-            _stream_ptr(stream)))
+            _current_stream(stream)))
 
     def check(self, stream=None) -> None:
-        check(_lib.molot_f8b_check(self._h, _stream_ptr(stream)))
+        check(_lib.molot_f8b_check(self._h, _current_stream(stream)))
 
     def evict(self, src, dst, budget, recent, kept, stream=None) -> None:
         """Moves the slots to keep from src to dst (pages of its own);
@@ -790,7 +823,7 @@ class F8Plan:
                 tuple(kept.shape) != (self.B, self.nkv, budget):
             raise ValueError("kept must be a contiguous int32 CUDA tensor [B][nkv][budget]")
         check(_lib.molot_f8b_evict(self._h, sp, dp, budget, recent, kept.data_ptr(),
-                                   _stream_ptr(stream)))
+                                   _current_stream(stream)))
 
 
 class PackedPlan:
@@ -823,7 +856,7 @@ class PackedPlan:
         self.ndocs = 0  # until it is built
         check(_lib.molot_packed_plan_build(self._h, arrays[0].size, nq, nkv, d,
                                            *(_ptr(a) for a in arrays), window,
-                                           _stream_ptr(stream)))
+                                           _current_stream(stream)))
         self.ndocs, self.nq, self.nkv, self.d = arrays[0].size, nq, nkv, d
         self.rows = int(arrays[0].sum())
         self.keys = self.rows if arrays[1] is None else int(arrays[1].sum())
@@ -843,10 +876,10 @@ class PackedPlan:
             self._h, qp, kp, vp, op,
             None if lse is None else _cuda_f32(lse, "lse", (self.rows, self.nq)), ty, qs, ks, vs,
             scale, softcap, None if slopes is None else _cuda_f32(slopes, "slopes", (self.nq,)),
-            _stream_ptr(stream)))
+            _current_stream(stream)))
 
     def check(self, stream=None) -> None:
-        check(_lib.molot_packed_check(self._h, _stream_ptr(stream)))
+        check(_lib.molot_packed_check(self._h, _current_stream(stream)))
 
 
 class Comm:

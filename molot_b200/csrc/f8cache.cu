@@ -5,7 +5,11 @@
 #include <algorithm>
 #include <cstdio>
 #include <cstring>
+#include <exception>
+#include <map>
+#include <mutex>
 #include <new>
+#include <tuple>
 #include <type_traits>
 #include <vector>
 
@@ -31,10 +35,35 @@ int f8_cuda(cudaError_t e, const char* what) {
     if (int rc_ = f8_cuda((call), #call)) return rc_;  \
   } while (0)
 
-constexpr int kF8MaxCtas = 2;  // decode CTAs per SM
+int f8_ctas(int d) { return d == 256 ? F8Dec<float, 256>::kCtas : F8Dec<float, 128>::kCtas; }
+
+// A launch that may start while the kernel before it drains (programmatic
+// dependent launch); the kernel waits for that one's end before it touches
+// anything but the plan.
+template <class... P, class... A>
+cudaError_t f8_launch(void (*kernel)(P...), dim3 grid, int threads, int smem, void* stream,
+                      int cluster, const A&... args) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute at[2] = {};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  c.attrs = at;
+  c.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&c, kernel, args...);
+}
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 size_t act_bytes(int t) { return t == MOLOT_ACT_F32 ? 4 : 2; }
+
+constexpr int kF8ClusterBlocks = 12;  // blocks per warp up to which clusters merge
+constexpr int kF8Straddle = 24;       // blocks that a second merge is worth
 
 // f(T{}, D) for an activation type and a head size.
 template <class F>
@@ -69,7 +98,9 @@ struct molot_f8b_plan {
   int* d_buf = nullptr;
   size_t h_cap = 0, d_cap = 0;  // ints
   cudaEvent_t uploaded = nullptr;
-  size_t o_prefix = 0, o_n0 = 0, o_len = 0, o_row = 0, o_blk = 0;  // F8Seq first
+  int grid = 0;     // decode CTAs
+  int cluster = 0;  // of so many CTAs
+  size_t o_ctas = 0, o_prefix = 0, o_n0 = 0, o_len = 0, o_row = 0, o_blk = 0;  // F8Seq first
   float* score = nullptr;  // accumulation scratch: scores, then [B][nq] lse
   size_t score_cap = 0;
   float* rec = nullptr;  // decode records, then tickets
@@ -85,6 +116,135 @@ struct molot_f8b_plan {
 
 namespace molot {
 namespace {
+
+// Decode clusters of `cluster` CTAs that device dev keeps resident at once
+// (the kernels of one head size share their shape; 0 when the query fails).
+int f8_resident(int d, int cluster, int dev) {
+  static std::mutex mu;
+  static std::map<std::tuple<int, int, int>, int> cache;
+  std::lock_guard<std::mutex> lk(mu);
+  const auto key = std::make_tuple(d, cluster, dev);
+  const auto hit = cache.find(key);
+  if (hit != cache.end()) return hit->second;
+  int n = 0;
+  auto query = [&](auto dd) {
+    constexpr int D = decltype(dd)::value;
+    const auto kernel = f8_decode_kernel<float, D>;
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         F8Dec<float, D>::kSmem);
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = cluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(cluster * 64);
+    c.blockDim = dim3(kF8Warps * 32);
+    c.dynamicSmemBytes = F8Dec<float, D>::kSmem;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &c) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+  };
+  if (d == 64) query(std::integral_constant<int, 64>{});
+  if (d == 128) query(std::integral_constant<int, 128>{});
+  if (d == 256) query(std::integral_constant<int, 256>{});
+  cache[key] = n;
+  return n;
+}
+
+// Shares of a decode, a CTA each; returns the cluster size (0: none).
+//
+// Few and short segments: a cluster per segment, merged in distributed
+// shared memory, when all the clusters are resident at once and a warp gets
+// at most kF8ClusterBlocks blocks.  One sequence of 4097 slots x 8 heads:
+// %CLUSTER% us, against %GLOBAL% us through records in global memory, whose
+// fence, ticket and loads take turns.
+// Else equal ranges of all items, or, where that leaves the longest range
+// within kF8Straddle blocks of it, ranges that end with the segments: a CTA
+// with parts of two segments merges twice.
+int f8_partition(const molot_f8b_plan* p, const std::vector<F8Seq>& seqs,
+                 const std::vector<int>& visit, int nkv, int HG, int d, std::vector<F8Cta>* out) {
+  const int B = (int)seqs.size();
+  const long long items = (long long)visit[B] * HG;
+  long long segs = 0;
+  int longest = 0;
+  for (const F8Seq& s : seqs) {
+    segs += s.nblk ? (long long)nkv * HG : 0;
+    longest = std::max(longest, s.nblk);
+  }
+  if (!items) {
+    out->assign(1, F8Cta{});
+    return 0;
+  }
+  for (const int C : {8, 16}) {
+    if (longest <= kF8Warps || longest > C * kF8Warps * (C == 8 ? 1 : kF8ClusterBlocks)) continue;
+    if (segs > f8_resident(d, C, p->device)) continue;
+    for (int b = 0; b < B; ++b)
+      for (int seg = 0; seg < (seqs[b].nblk ? nkv * HG : 0); ++seg)
+        for (int r = 0; r < C; ++r) {
+          const int i0 = (int)((long long)seqs[b].nblk * r / C);
+          const int i1 = (int)((long long)seqs[b].nblk * (r + 1) / C);
+          out->push_back(F8Cta{b, seg, i0, i1 - i0, 0, 1, 0, 1});
+        }
+    return C;
+  }
+  const int max_grid = f8_ctas(d) * p->sms;
+  // ranges that end with the segments
+  const long long even = (items + max_grid - 1) / max_grid;
+  long long need = 0, longest_share = 0;
+  auto parts = [&](int nblk) {
+    return (int)std::max<long long>(
+        1, std::min<long long>((long long)nblk * max_grid / items, (nblk + kF8Warps - 1) / kF8Warps));
+  };
+  for (const F8Seq& s : seqs)
+    if (s.nblk) {
+      need += (long long)parts(s.nblk) * nkv * HG;
+      longest_share = std::max<long long>(longest_share, (s.nblk + parts(s.nblk) - 1) / parts(s.nblk));
+    }
+  if (need <= max_grid && longest_share <= even + kF8Straddle) {
+    for (int b = 0; b < B; ++b) {
+      const int k = seqs[b].nblk ? parts(seqs[b].nblk) : 0;
+      for (int seg = 0; seg < (k ? nkv * HG : 0); ++seg) {
+        const int c0 = (int)out->size();
+        for (int r = 0; r < k; ++r) {
+          const int i0 = (int)((long long)seqs[b].nblk * r / k);
+          const int i1 = (int)((long long)seqs[b].nblk * (r + 1) / k);
+          out->push_back(F8Cta{b, seg, i0, i1 - i0, 2 * c0, k, 2 * c0, k});
+        }
+      }
+    }
+    return 0;
+  }
+  const long long grid = std::min<long long>((items + kF8Warps - 1) / kF8Warps, max_grid);
+  out->resize(grid);
+  auto start = [&](long long c) { return c * items / grid; };
+  auto owner = [&](long long x) { return ((x + 1) * grid + items - 1) / items - 1; };
+  int b = 0;
+  for (long long c = 0; c < grid; ++c) {
+    F8Cta& k = (*out)[c];
+    k = F8Cta{};
+    const long long x0 = start(c), x1 = start(c + 1);
+    k.items = (int)(x1 - x0);
+    // the segment of item x, and who shares it
+    auto locate = [&](long long x, int* seg, int* i0, int* rec, int* n) {
+      while ((long long)visit[b + 1] * HG <= x) ++b;
+      const long long base = (long long)visit[b] * HG, nblk = seqs[b].nblk;
+      *seg = (int)((x - base) / nblk);
+      *i0 = (int)((x - base) % nblk);
+      const long long y0 = base + *seg * nblk, c0 = owner(y0);
+      *rec = (int)(2 * c0 + (start(c0) == y0 ? 0 : 1));
+      *n = (int)(owner(y0 + nblk - 1) - c0 + 1);
+    };
+    int seg, i0;
+    locate(x0, &k.seg, &k.i0, &k.rec_first, &k.n_first);
+    k.b = b;
+    locate(x1 - 1, &seg, &i0, &k.rec_last, &k.n_last);
+  }
+  return 0;
+}
 
 int f8_build(molot_f8b_plan* p, int B, int nq, int nkv, int d, const int* seq_lens,
              const int* new_lens, const int* starts, const int* prefix, int window,
@@ -132,7 +292,12 @@ int f8_build(molot_f8b_plan* p, int B, int nq, int nkv, int d, const int* seq_le
   visit[B] = (int)nv;
   row[B] = (int)nr;
   blk[B] = (int)nb;
-  const size_t o_prefix = (size_t)B * (sizeof(F8Seq) / 4), o_n0 = o_prefix + B + 1,
+  const int HG = (nq / nkv + 7) / 8;
+  std::vector<F8Cta> ctas;
+  const int cluster = f8_partition(p, seqs, visit, nkv, HG, d, &ctas);
+  const int grid = (int)ctas.size();
+  const size_t o_ctas = (size_t)B * (sizeof(F8Seq) / 4),
+               o_prefix = o_ctas + (size_t)grid * (sizeof(F8Cta) / 4), o_n0 = o_prefix + B + 1,
                o_len = o_n0 + B, o_row = o_len + B, o_blk = o_row + B + 1,
                total = o_blk + B + 1;
   if (p->built) F8_CUDA(cudaEventSynchronize(p->uploaded));  // staging still being read?
@@ -154,7 +319,7 @@ int f8_build(molot_f8b_plan* p, int B, int nq, int nkv, int d, const int* seq_le
     p->d_cap = cap;
   }
   // decode scratch: two records a CTA, a ticket per segment
-  const size_t rec = (size_t)2 * kF8MaxCtas * p->sms * (8 * (size_t)d + 16);
+  const size_t rec = (size_t)2 * f8_ctas(d) * p->sms * (8 * (size_t)d + 16);
   const size_t tickets = (size_t)B * nkv * ((nq / nkv + 7) / 8);
   if (p->rec_cap < rec || p->tickets_cap < tickets) {
     F8_CUDA(cudaDeviceSynchronize());
@@ -176,6 +341,7 @@ int f8_build(molot_f8b_plan* p, int B, int nq, int nkv, int d, const int* seq_le
     }
   }
   std::memcpy(p->h_buf, seqs.data(), B * sizeof(F8Seq));
+  std::memcpy(p->h_buf + o_ctas, ctas.data(), grid * sizeof(F8Cta));
   std::memcpy(p->h_buf + o_prefix, visit.data(), (B + 1) * sizeof(int));
   std::memcpy(p->h_buf + o_n0, n0.data(), B * sizeof(int));
   std::memcpy(p->h_buf + o_len, len.data(), B * sizeof(int));
@@ -183,6 +349,9 @@ int f8_build(molot_f8b_plan* p, int B, int nq, int nkv, int d, const int* seq_le
   std::memcpy(p->h_buf + o_blk, blk.data(), (B + 1) * sizeof(int));
   F8_CUDA(cudaMemcpyAsync(p->d_buf, p->h_buf, total * sizeof(int), cudaMemcpyHostToDevice, st));
   F8_CUDA(cudaEventRecord(p->uploaded, st));
+  p->grid = grid;
+  p->cluster = cluster;
+  p->o_ctas = o_ctas;
   p->o_prefix = o_prefix;
   p->o_n0 = o_n0;
   p->o_len = o_len;
@@ -324,9 +493,9 @@ int molot_f8b_write(molot_f8b_plan* p, const molot_f8b_layer* layer, const void*
   const F8WriteArgs a{pool, k, v, k_stride, v_stride, p->d_buf + p->o_n0, p->d_buf + p->o_len,
                       p->d_buf + p->o_row, p->d_buf + p->o_blk, layer->weight, p->B, p->touched * p->nkv * 2};
   return f8_dispatch(act_dtype, p->d, [&](auto t, auto dd) {
-    f8_write_kernel<decltype(t), decltype(dd)::value>
-        <<<(a.nitems + 3) / 4, 128, 0, (cudaStream_t)stream>>>(a);
-    return f8_cuda(cudaGetLastError(), "f8 write launch");
+    return f8_cuda(f8_launch(f8_write_kernel<decltype(t), decltype(dd)::value>, (a.nitems + 3) / 4,
+                             128, 0, stream, 0, a),
+                   "f8 write launch");
   });
 }
 
@@ -362,6 +531,7 @@ int molot_f8b_decode(molot_f8b_plan* p, const molot_f8b_layer* layer, const void
   F8DecodeArgs a{};
   a.pool = pool;
   a.seqs = p->seqs();
+  a.ctas = reinterpret_cast<const F8Cta*>(p->d_buf + p->o_ctas);
   a.prefix = p->d_buf + p->o_prefix;
   a.q = q;
   a.o = o;
@@ -376,7 +546,7 @@ int molot_f8b_decode(molot_f8b_plan* p, const molot_f8b_layer* layer, const void
   a.nq = p->nq;
   a.G = G;
   a.HG = (G + 7) / 8;
-  a.items = p->visits * a.HG;
+  a.cluster = p->cluster;
   a.has_empty = p->has_empty;
   a.status = p->status;
   a.timeout_ns = kF8WaitNs;
@@ -391,11 +561,10 @@ int molot_f8b_decode(molot_f8b_plan* p, const molot_f8b_layer* layer, const void
         if (F::kSmem > 48 * 1024)
           F8_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        F::kSmem));
-        static_assert(F::kCtas <= kF8MaxCtas, "records");
-        const int grid = (int)std::max<long long>(
-            1, std::min<long long>(a.items, (long long)F::kCtas * p->sms));
-        kernel<<<grid, kF8Warps * 32, F::kSmem, (cudaStream_t)stream>>>(mk, mv, a);
-        return f8_cuda(cudaGetLastError(), "f8 decode launch");
+        if (p->cluster > 8)
+          F8_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        return f8_cuda(f8_launch(kernel, p->grid, kF8Warps * 32, F::kSmem, stream, p->cluster, mk, mv, a),
+                       "f8 decode launch");
       }))
     return rc;
   if (!weight_out || !p->max_len) return MOLOT_OK;

@@ -41,6 +41,15 @@ struct alignas(16) F8Seq {
   int nblk;      // blocks to visit in all: na + the window's
 };
 
+// One decode CTA's range of a plan (device array): it starts at block i0 of
+// segment seg (kv head, head group) of sequence b and takes `items` blocks.
+// Where its first or last segment is shared with other CTAs: the first of
+// their records (2 * CTA, + 1 for a CTA's second one) and how many they are.
+struct alignas(16) F8Cta {
+  int b, seg, i0, items;
+  int rec_first, n_first, rec_last, n_last;
+};
+
 // A pool's device pointers (one layer).
 struct F8Pool {
   uint8_t* k;
@@ -107,6 +116,7 @@ __global__ void __launch_bounds__(128) f8_write_kernel(const __grid_constant__ F
   const int kv = item & 1, h = (item >> 1) % nkv, x = (item >> 1) / nkv;
   const int b = warp_find(a.blk, a.B, x);
   const int n0 = a.n0[b], n = a.len[b];
+  ptx::pdl_wait();
   const int blk = n0 / kF8Blk + (x - a.blk[b]);
   const int t0 = blk * kF8Blk;  // first slot of the block
   const int ps = a.pool.page_size;
@@ -197,6 +207,7 @@ __global__ void __launch_bounds__(128) f8_write_kernel(const __grid_constant__ F
 struct F8DecodeArgs {
   F8Pool pool;
   const F8Seq* seqs;
+  const F8Cta* ctas;
   const int* prefix;  // [B + 1] block visits (a block once for every kv head)
   const void* q;      // sequence b, head h: q + b * q_stride + h * d
   void* o;            // [B][nq][d]
@@ -207,8 +218,8 @@ struct F8DecodeArgs {
   float* rec;    // [2 * grid] records
   int* tickets;  // [B * nkv * head groups], zero between launches
   long long q_stride;
-  long long items;
   int B, nq, G, HG;  // HG head groups of up to 8 per kv head
+  int cluster;       // CTAs of a cluster, a segment each; 0: records in global memory
   int has_empty;     // some sequence sees nothing
   int* status;       // 1 after a bounded wait ran out
   unsigned long long timeout_ns;
@@ -234,7 +245,9 @@ struct F8Dec {
   static constexpr int kRec = kFrag + 16;    // + M[8], l[8]
   static constexpr int kQ = KS * 32 * 8;     // bytes of one FP16 part of Q
   static constexpr int kBar = kRing + 2 * kQ + 64;
-  static constexpr int kSmem = kBar + kF8Warps * kStages * 8 + 1024;  // + alignment
+  // what a cluster's CTAs send here: 1 / C of each one's positions, M, l
+  static constexpr int kPush = kBar + kF8Warps * kStages * 8;
+  static constexpr int kSmem = kPush + kFrag * 4 + 16 * 64 + 1024;  // + alignment
   static_assert(kRing >= kF8Warps * kRec * 4, "the warps' records take the ring's place");
 };
 
@@ -306,8 +319,7 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;  // fragment row group, column pair
   const int nkv = a.pool.nkv, ps = a.pool.page_size, bpp = ps / kF8Blk;
-  const long long grid = gridDim.x;
-  const long long x0 = blockIdx.x * a.items / grid, x1 = (blockIdx.x + 1) * a.items / grid;
+  const F8Cta cta = a.ctas[blockIdx.x];
   const uint32_t ring = ptx::smem_u32(smem) + warp * F::kStages * F::kBlk;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + F::kBar) + warp * F::kStages;
   // Where this lane's pieces lie in a box: rows of HB bytes, the 16-byte
@@ -315,26 +327,29 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
   auto piece = [&](int r, int c) {
     return r * F::HB + ((c ^ (F::HB == 128 ? r & 7 : (r >> 1) & 3)) * 16);
   };
-  int count = 0, put = 0;  // blocks this warp has waited for, and asked for
+  // stages and phases of the blocks this warp waits for and asks for next
+  int st_get = 0, st_put = 0, phase = 0, asked = 0;
   if (lane == 0)
     for (int i = 0; i < F::kStages; ++i) ptx::mbar_init(full + i, 1);
   if (tid == 0) s_abort = 0;
   ptx::fence_mbar_init();
+  if (a.cluster) ptx::cluster_arrive();
+  int b = cta.b, seg = cta.seg, i0 = cta.i0, left = cta.items;
+  F8Seq sq = a.seqs[b];
+  // What the plan uploaded is there; q, the pools and the scratch may be the
+  // preceding kernel's.
+  ptx::pdl_wait();
+  ptx::pdl_launch_dependents();
   __syncthreads();
 
-  for (long long x = x0; x < x1;) {
-    // the item's segment
-    const int b = warp_find(a.prefix, a.B, (int)(x / a.HG));
-    const F8Seq sq = a.seqs[b];
-    const long long base = (long long)a.prefix[b] * a.HG;
-    const int seg = (int)((x - base) / sq.nblk);
-    const int i0 = (int)((x - base) % sq.nblk);
-    const int i1 = (int)min((long long)sq.nblk, i0 + (x1 - x));
+  // (a CTA of a cluster takes part in its merge even without blocks)
+  for (bool go = left > 0 || a.cluster; go; go = left > 0) {
+    const int i1 = min(sq.nblk, i0 + left);
     const int h = seg / a.HG, hg = seg % a.HG;
     const int head0 = h * a.G + hg * 8, nh = min(8, a.G - hg * 8);
     const int* bt = a.pool.bt + (long long)b * a.pool.max_pages;
-    const bool first_piece = x == x0;
-    x += i1 - i0;
+    const bool first_piece = left == cta.items;
+    left -= i1 - i0;
 
     // The warp's blocks are i0 + warp + 8 m, m in [0, nm).  They are fetched
     // kStages ahead; of a run of 32, lane l has block l's place and scales.
@@ -359,16 +374,16 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
         }
       }
       if (lane == (m & 31)) {
-        const int st = put % F::kStages;
-        const uint32_t dst = ring + st * F::kBlk;
-        ptx::mbar_arrive_expect_tx(full + st, F::kBlk);
+        const uint32_t dst = ring + st_put * F::kBlk;
+        ptx::mbar_arrive_expect_tx(full + st_put, F::kBlk);
 #pragma unroll
         for (int i = 0; i < NH; ++i) {
-          tma_rows(dst + i * kF8Blk * 128, &mk, i * 128, place * kF8Blk, full + st);
-          tma_rows(dst + kF8Blk * D + i * kF8Blk * 128, &mv, i * 128, place * kF8Blk, full + st);
+          tma_rows(dst + i * kF8Blk * 128, &mk, i * 128, place * kF8Blk, full + st_put);
+          tma_rows(dst + kF8Blk * D + i * kF8Blk * 128, &mv, i * 128, place * kF8Blk, full + st_put);
         }
       }
-      ++put;
+      st_put = st_put + 1 == F::kStages ? 0 : st_put + 1;
+      ++asked;
     };
 #pragma unroll
     for (int m = 0; m < F::kStages; ++m)
@@ -424,14 +439,13 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
       if ((m & 31) == 0) ks_run = ks_in, vs_run = vs_in;
       const float ksc = __shfl_sync(0xffffffffu, ks_run, m & 31);
       const float vsc = __shfl_sync(0xffffffffu, vs_run, m & 31);
-      const int st = count % F::kStages;
-      const uint32_t src = ring + st * F::kBlk, vsrc = src + kF8Blk * D;
-      if (!s_abort && !ptx::mbar_wait_bounded(full + st, (count / F::kStages) & 1, a.timeout_ns)) {
+      const uint32_t src = ring + st_get * F::kBlk, vsrc = src + kF8Blk * D;
+      if (!s_abort && !ptx::mbar_wait_bounded(full + st_get, phase, a.timeout_ns)) {
         s_abort = 1;
         atomicCAS(a.status, 0, 1);
       }
       __syncwarp();
-      ++count;
+      if (++st_get == F::kStages) st_get = 0, phase ^= 1;
       // S^T: two chains, so that a product need not wait for the last one
       float s[2][4] = {};
 #pragma unroll
@@ -611,8 +625,12 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
         }
       }
     };
-    const bool whole = i0 == 0 && i1 == sq.nblk;
+    const bool whole = !a.cluster && i0 == 0 && i1 == sq.nblk;
     float* rec = a.rec + (2 * (long long)blockIdx.x + (first_piece ? 0 : 1)) * F::kRec;
+    // a cluster's CTA r merges positions [r * per, (r + 1) * per)
+    const int C = a.cluster, per = C ? np / C : 0;
+    const uint32_t push = ptx::smem_u32(smem + F::kPush), rank = C ? ptx::cluster_ctarank() : 0;
+    if (C) ptx::cluster_wait();  // every CTA of the cluster has started
     for (int i = tid; i < np; i += kThreads) {
       const int f4 = position(i), hh = 2 * (f4 & 3);
       float2 mm = make_float2(-CUDART_INF_F, -CUDART_INF_F), ll = make_float2(0.f, 0.f);
@@ -636,6 +654,12 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
       }
       if (whole) {
         finish(f4, acc, mm, ll);
+      } else if (C) {
+        const int to = i / per;
+        ptx::st_dsmem4(push + (rank * per + i % per) * 16, to, acc);
+        if (i % per < 4)  // M, l of the heads 2 hh', 2 hh' + 1, hh' < th; per is at least th
+          ptx::st_dsmem4(push + F::kFrag * 4 + rank * 64 + (f4 & 3) * 16, to,
+                         make_float4(mm.x, mm.y, ll.x, ll.y));
       } else {
         reinterpret_cast<float4*>(rec)[f4] = acc;
         if (f4 < 4) {
@@ -644,12 +668,37 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
         }
       }
     }
-    if (!whole) {
-      // CTAs [c0, c1] share the segment's items [y0, y1]
-      const long long y0 = base + (long long)seg * sq.nblk, y1 = y0 + sq.nblk - 1;
-      const long long c0 = ((y0 + 1) * grid + a.items - 1) / a.items - 1;
-      const long long c1 = ((y1 + 1) * grid + a.items - 1) / a.items - 1;
-      const int n = (int)(c1 - c0) + 1;
+    if (C) {
+      // The positions sent here, a CTA's per lane: sums by shuffles.
+      ptx::cluster_sync();
+      const int k = tid & (C - 1);
+      for (int i = tid / C; i < (per + 31) / 32 * 32; i += kThreads / C) {
+        const int li = min(i, per - 1), f4 = position(rank * per + li);
+        const float4 v = *reinterpret_cast<const float4*>(smem + F::kPush + (k * per + li) * 16);
+        const float4 st = *reinterpret_cast<const float4*>(smem + F::kPush + F::kFrag * 4 + k * 64 +
+                                                           (f4 & 3) * 16);
+        float2 mm = make_float2(st.x, st.y);
+        for (int x = 1; x < C; x <<= 1) {
+          mm.x = fmaxf(mm.x, __shfl_xor_sync(0xffffffffu, mm.x, x));
+          mm.y = fmaxf(mm.y, __shfl_xor_sync(0xffffffffu, mm.y, x));
+        }
+        const float fx = st.x == -CUDART_INF_F ? 0.f : ex2(st.x - mm.x);
+        const float fy = st.y == -CUDART_INF_F ? 0.f : ex2(st.y - mm.y);
+        float4 acc = make_float4(fx * v.x, fy * v.y, fx * v.z, fy * v.w);
+        float2 ll = make_float2(fx * st.z, fy * st.w);
+        for (int x = 1; x < C; x <<= 1) {
+          acc.x += __shfl_xor_sync(0xffffffffu, acc.x, x);
+          acc.y += __shfl_xor_sync(0xffffffffu, acc.y, x);
+          acc.z += __shfl_xor_sync(0xffffffffu, acc.z, x);
+          acc.w += __shfl_xor_sync(0xffffffffu, acc.w, x);
+          ll.x += __shfl_xor_sync(0xffffffffu, ll.x, x);
+          ll.y += __shfl_xor_sync(0xffffffffu, ll.y, x);
+        }
+        if (k == 0 && i < per) finish(f4, acc, mm, ll);
+      }
+    } else if (!whole) {
+      const int rec0 = first_piece ? cta.rec_first : cta.rec_last;
+      const int n = first_piece ? cta.n_first : cta.n_last;
       __threadfence();
       __syncthreads();
       if (tid == 0) {
@@ -661,10 +710,10 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
       __syncthreads();
       if (s_last) {
         __threadfence();
-        // The first CTA's record is its first one when the segment starts
-        // its range, else its last; the others' ranges start inside.
-        const int off0 = c0 * a.items / grid == y0 ? 0 : 1;
-        auto record = [&](int k) { return a.rec + (2 * (c0 + k) + (k ? 0 : off0)) * F::kRec; };
+        // records of the CTAs after the first are their first ones
+        auto record = [&](int k) {
+          return a.rec + (long long)(k ? (rec0 & ~1) + 2 * k : rec0) * F::kRec;
+        };
         // factors of the records: [n][8] M, then l, then the heads' M, l
         float* fac = reinterpret_cast<float*>(smem);
         float* fl = fac + n * 8;
@@ -728,9 +777,17 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
     // shared memory is free for the next segment's copies
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
+    if (left > 0) {  // the next segment, of the next sequence that sees anything
+      i0 = 0;
+      if (++seg == nkv * a.HG) {
+        seg = 0;
+        do sq = a.seqs[++b];
+        while (sq.nblk == 0);
+      }
+    }
   }
   if (s_abort)  // copies in flight end before the CTA does
-    for (int k = max(0, put - F::kStages); k < put; ++k)
+    for (int k = max(0, asked - F::kStages); k < asked; ++k)
       ptx::mbar_wait_bounded(full + k % F::kStages, (k / F::kStages) & 1, a.timeout_ns);
   if (a.has_empty)
     for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
