@@ -493,9 +493,9 @@ int molot_f8b_write(molot_f8b_plan* p, const molot_f8b_layer* layer, const void*
   const F8WriteArgs a{pool, k, v, k_stride, v_stride, p->d_buf + p->o_n0, p->d_buf + p->o_len,
                       p->d_buf + p->o_row, p->d_buf + p->o_blk, layer->weight, p->B, p->touched * p->nkv * 2};
   return f8_dispatch(act_dtype, p->d, [&](auto t, auto dd) {
-    return f8_cuda(f8_launch(f8_write_kernel<decltype(t), decltype(dd)::value>, (a.nitems + 3) / 4,
-                             128, 0, stream, 0, a),
-                   "f8 write launch");
+    f8_write_kernel<decltype(t), decltype(dd)::value>
+        <<<(a.nitems + 3) / 4, 128, 0, (cudaStream_t)stream>>>(a);
+    return f8_cuda(cudaGetLastError(), "f8 write launch");
   });
 }
 
@@ -570,8 +570,10 @@ int molot_f8b_decode(molot_f8b_plan* p, const molot_f8b_layer* layer, const void
   if (!weight_out || !p->max_len) return MOLOT_OK;
   const F8WeightArgs w{pool, p->seqs(), p->d_buf + p->o_prefix, p->score, lse2, layer->weight,
                        weight_out, p->nq, G};
-  f8_weight_kernel<<<dim3((p->max_len + 127) / 128, p->nkv, p->B), 128, 0, (cudaStream_t)stream>>>(w);
-  return f8_cuda(cudaGetLastError(), "f8 weight launch");
+  const int per = 128 * kF8WeightSlots;
+  return f8_cuda(f8_launch(f8_weight_kernel, dim3((p->max_len + per - 1) / per, p->nkv, p->B), 128,
+                           0, stream, 0, w),
+                 "f8 weight launch");
 }
 
 int molot_f8b_evict(molot_f8b_plan* p, const molot_f8b_layer* src, const molot_f8b_layer* dst,
@@ -582,6 +584,7 @@ int molot_f8b_evict(molot_f8b_plan* p, const molot_f8b_layer* src, const molot_f
   if (int rc = f8_pool(p, src, p ? p->max_len : 0, &a.src)) return rc;
   if (int rc = f8_pool(p, dst, std::min(p->max_len, budget), &a.dst)) return rc;
   if (!src->weight || !dst->weight || !kept) return f8_fail(MOLOT_ERR_INVALID, "null pointer");
+  if (!aligned16(src->weight)) return f8_fail(MOLOT_ERR_INVALID, "counters must be 16-byte aligned");
   a.win = src->weight;
   a.wout = dst->weight;
   a.kept = kept;
@@ -589,17 +592,18 @@ int molot_f8b_evict(molot_f8b_plan* p, const molot_f8b_layer* src, const molot_f
   a.B = p->B;
   a.budget = budget;
   a.recent = recent;
-  f8_select_kernel<<<dim3(p->nkv, p->B), kF8SelThreads, 0, (cudaStream_t)stream>>>(a);
-  F8_CUDA(cudaGetLastError());
+  const int keys = std::min(std::max(p->max_len - recent, 0), kF8SelKeys);
+  const int smem = (keys + 3) / 4 * 16;
+  F8_CUDA(cudaFuncSetAttribute(f8_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               kF8SelKeys * 4));
+  F8_CUDA(f8_launch(f8_select_kernel, dim3(p->nkv, p->B), kF8SelThreads, smem, stream, 0, a));
   const int blocks = (std::min(p->max_len, budget) + kF8Blk - 1) / kF8Blk;
   if (!blocks) return MOLOT_OK;
-  const dim3 grid((blocks * p->nkv * 2 + 3) / 4, p->B);
-  switch (p->d) {
-    case 64: f8_move_kernel<64><<<grid, 128, 0, (cudaStream_t)stream>>>(a); break;
-    case 128: f8_move_kernel<128><<<grid, 128, 0, (cudaStream_t)stream>>>(a); break;
-    default: f8_move_kernel<256><<<grid, 128, 0, (cudaStream_t)stream>>>(a); break;
-  }
-  return f8_cuda(cudaGetLastError(), "f8 move launch");
+  const dim3 grid((blocks * p->nkv + 3) / 4, p->B);
+  const auto move = p->d == 64    ? f8_move_kernel<64>
+                    : p->d == 128 ? f8_move_kernel<128>
+                                  : f8_move_kernel<256>;
+  return f8_cuda(f8_launch(move, grid, 128, 0, stream, 0, a), "f8 move launch");
 }
 
 int molot_f8b_check(molot_f8b_plan* p, void* stream) {

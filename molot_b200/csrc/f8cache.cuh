@@ -116,7 +116,6 @@ __global__ void __launch_bounds__(128) f8_write_kernel(const __grid_constant__ F
   const int kv = item & 1, h = (item >> 1) % nkv, x = (item >> 1) / nkv;
   const int b = warp_find(a.blk, a.B, x);
   const int n0 = a.n0[b], n = a.len[b];
-  ptx::pdl_wait();
   const int blk = n0 / kF8Blk + (x - a.blk[b]);
   const int t0 = blk * kF8Blk;  // first slot of the block
   const int ps = a.pool.page_size;
@@ -499,8 +498,15 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
         const int i = i0 + warp + kF8Warps * m;
         float* sp = a.score + (((long long)a.prefix[b] + (long long)h * sq.nblk + i) * kF8Blk + g) *
                                   a.G + hg * 8 + 2 * t4;
-        if (2 * t4 < nh) sp[0] = z[0], sp[8 * a.G] = z[2];
-        if (2 * t4 + 1 < nh) sp[1] = z[1], sp[8 * a.G + 1] = z[3];
+        if (a.G % 2 == 0) {
+          if (2 * t4 < nh) {
+            *reinterpret_cast<float2*>(sp) = make_float2(z[0], z[1]);
+            *reinterpret_cast<float2*>(sp + 8 * a.G) = make_float2(z[2], z[3]);
+          }
+        } else {
+          if (2 * t4 < nh) sp[0] = z[0], sp[8 * a.G] = z[2];
+          if (2 * t4 + 1 < nh) sp[1] = z[1], sp[8 * a.G + 1] = z[3];
+        }
       }
       const float ev = (float)((int)(__float_as_uint(vsc) >> 23) - 127);
       const float q0 = fmaxf(z[0], z[2]) + ev, q1 = fmaxf(z[1], z[3]) + ev;
@@ -812,29 +818,69 @@ struct F8WeightArgs {
   int nq, G;
 };
 
+constexpr int kF8WeightSlots = 4;  // slots per thread of the counter kernel
+
 // Counters: wout = win + the slot's weights summed over the kv head's group,
-// from the scores that the decode left.  A thread per slot; heads in order,
-// so the sum does not depend on the launch.
+// from the scores that the decode left.  Heads are summed in order, so the
+// sum does not depend on the launch.  Bound by the scores' bytes; each thread
+// has its slots' loads in flight together.
 __global__ void __launch_bounds__(128) f8_weight_kernel(const __grid_constant__ F8WeightArgs a) {
   const int g = blockIdx.y, b = blockIdx.z;
   const F8Seq sq = a.seqs[b];
-  const int t = blockIdx.x * 128 + threadIdx.x;
-  if (t >= sq.n) return;
-  const int ps = a.pool.page_size;
-  const long long hp =
-      (long long)a.pool.bt[(long long)b * a.pool.max_pages + t / ps] * a.pool.nkv + g;
-  const int blk = t / kF8Blk;
-  const bool inA = blk >= sq.a0 && blk < sq.a0 + sq.na;
-  const int i = inA ? blk - sq.a0 : blk - sq.b0 + sq.na;
-  float p = 0.f;
-  if (inA || (blk >= sq.b0 && i < sq.nblk)) {
-    const float* s = a.score +
-                     (((long long)a.prefix[b] + (long long)g * sq.nblk + i) * kF8Blk + t % kF8Blk) * a.G;
-    const float* z = a.lse2 + (long long)b * a.nq + (long long)g * a.G;
-    for (int j = 0; j < a.G; ++j)
-      if (s[j] != -CUDART_INF_F) p += ex2(s[j] - z[j]);
+  const int first = blockIdx.x * (128 * kF8WeightSlots) + threadIdx.x;
+  ptx::pdl_wait();
+  if (first >= sq.n) return;
+  const int ps = a.pool.page_size, nkv = a.pool.nkv, G = a.G;
+  const int* bt = a.pool.bt + (long long)b * a.pool.max_pages;
+  const long long visit0 = (long long)a.prefix[b] + (long long)g * sq.nblk;
+  const float* z = a.lse2 + (long long)b * a.nq + (long long)g * G;
+  const float* s[kF8WeightSlots];  // the slot's scores, NULL where it was not visited
+  long long at[kF8WeightSlots];
+  float w[kF8WeightSlots];
+#pragma unroll
+  for (int i = 0; i < kF8WeightSlots; ++i) {
+    const int t = first + 128 * i;
+    s[i] = nullptr;
+    at[i] = -1;
+    if (t >= sq.n) continue;
+    const int page = t / ps;
+    at[i] = ((long long)bt[page] * nkv + g) * ps + t - page * ps;
+    w[i] = a.win[at[i]];
+    const int blk = t / kF8Blk;
+    const bool in_a = blk >= sq.a0 && blk < sq.a0 + sq.na;
+    const int v = in_a ? blk - sq.a0 : blk - sq.b0 + sq.na;
+    if (in_a || (blk >= sq.b0 && v < sq.nblk))
+      s[i] = a.score + ((visit0 + v) * kF8Blk + t % kF8Blk) * G;
   }
-  a.wout[hp * ps + t % ps] = a.win[hp * ps + t % ps] + p;
+  float p[kF8WeightSlots] = {};
+  if (G % 4 == 0) {
+    for (int j = 0; j < G; j += 4) {
+      float4 v[kF8WeightSlots];
+#pragma unroll
+      for (int i = 0; i < kF8WeightSlots; ++i)
+        v[i] = s[i] ? *reinterpret_cast<const float4*>(s[i] + j)
+                    : make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
+      const float z0 = z[j], z1 = z[j + 1], z2 = z[j + 2], z3 = z[j + 3];
+#pragma unroll
+      for (int i = 0; i < kF8WeightSlots; ++i) {
+        // a slot that is not seen has -inf; a sequence that sees nothing has
+        // no visited slots
+        p[i] += ex2(v[i].x - z0);
+        p[i] += ex2(v[i].y - z1);
+        p[i] += ex2(v[i].z - z2);
+        p[i] += ex2(v[i].w - z3);
+      }
+    }
+  } else {
+    for (int j = 0; j < G; ++j) {
+#pragma unroll
+      for (int i = 0; i < kF8WeightSlots; ++i)
+        if (s[i]) p[i] += ex2(s[i][j] - z[j]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kF8WeightSlots; ++i)
+    if (at[i] >= 0) a.wout[at[i]] = w[i] + (s[i] ? p[i] : 0.f);
 }
 
 // ------------------------------------------------------------------ evict
@@ -855,146 +901,278 @@ __device__ __forceinline__ uint32_t f8_key(float w) {
 }
 
 constexpr int kF8SelThreads = 1024;
+constexpr int kF8SelHists = 8;  // copies of the histogram: the leading digits of weights are few
+// Keys that a CTA keeps in shared memory; longer sequences read them again
+// from the pool in every pass.
+constexpr int kF8SelKeys = 48 * 1024;
 
 // The slots to keep of one sequence and kv head, ascending: a radix select
 // of the (budget - recent)-th largest key over slots [0, n - recent), 8 bits
-// a pass, then an ordered compaction: keys above the threshold, and the
-// lowest slots among those equal to it.
+// a pass until a bucket is taken whole, then an ordered compaction: keys above the threshold, and the
+// lowest slots among those equal to it.  One sequence of 4351 slots x 8
+// heads, and 16 of up to 32768, took 37 and 95 us with the keys read from
+// the pool in each pass and one thread walking the histogram.
 __global__ void __launch_bounds__(kF8SelThreads) f8_select_kernel(const __grid_constant__ F8EvictArgs a) {
+  extern __shared__ uint32_t keys[];
   const int g = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n = a.seqs[b].n, nkv = a.src.nkv, ps = a.src.page_size;
   int* kept = a.kept + ((long long)b * nkv + g) * a.budget;
+  ptx::pdl_wait();
+  ptx::pdl_launch_dependents();
   if (n <= a.budget) {
     for (int i = tid; i < a.budget; i += kF8SelThreads) kept[i] = i < n ? i : -1;
     return;
   }
   const int old = n - a.recent, want = a.budget - a.recent;
+  for (int i = tid; i < a.recent; i += kF8SelThreads) kept[want + i] = old + i;
+  if (want == 0) return;
   const int* bt = a.src.bt + (long long)b * a.src.max_pages;
-  auto key = [&](int t) {
-    return f8_key(a.win[((long long)bt[t / ps] * nkv + g) * ps + t % ps]);
+  // four keys of slots t .. t + 3, t a multiple of 4 (pages and blocks are)
+  auto load4 = [&](int t) {
+    const int page = t / ps;
+    const float4 w = *reinterpret_cast<const float4*>(
+        a.win + ((long long)bt[page] * nkv + g) * ps + t - page * ps);
+    return make_uint4(f8_key(w.x), f8_key(w.y), f8_key(w.z), f8_key(w.w));
   };
-  __shared__ int hist[256];
-  __shared__ int s_digit, s_left;
+  const bool held = old <= kF8SelKeys;
+  if (held) {
+#pragma unroll 4
+    for (int t = 4 * tid; t < old; t += 4 * kF8SelThreads)
+      *reinterpret_cast<uint4*>(keys + t) = load4(t);
+    __syncthreads();
+  }
+  auto key4 = [&](int t) { return held ? *reinterpret_cast<const uint4*>(keys + t) : load4(t); };
+  __shared__ int hist[kF8SelHists][256];
+  __shared__ int s_digit, s_left, s_count;
   uint32_t pre = 0, mask = 0;
   int left = want;  // still to take among the keys that match the prefix
-  for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    for (int i = tid; i < kF8SelHists * 256; i += kF8SelThreads) (&hist[0][0])[i] = 0;
     __syncthreads();
-    for (int t = tid; t < old; t += kF8SelThreads) {
-      const uint32_t k = key(t);
-      if ((k & mask) == pre) atomicAdd(&hist[(k >> shift) & 255], 1);
+    for (int t = 4 * tid; t < old; t += 4 * kF8SelThreads) {
+      const uint4 k4 = key4(t);
+      const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (t + i < old && (k[i] & mask) == pre)
+          atomicAdd(&hist[warp % kF8SelHists][(k[i] >> shift) & 255], 1);
     }
     __syncthreads();
-    if (tid == 0) {
-      int r = left, dgt = 255;
-      while (dgt > 0 && hist[dgt] < r) r -= hist[dgt--];
-      s_digit = dgt;
-      s_left = r;
+    if (warp == 0) {
+      // lane l: bins 255 - 8 l down to 248 - 8 l; the digit is where the
+      // count from the top reaches `left`
+      int c[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        c[i] = 0;
+#pragma unroll
+        for (int k = 0; k < kF8SelHists; ++k) c[i] += hist[k][255 - 8 * lane - i];
+        sum += c[i];
+      }
+      int incl = sum;
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, x);
+        if (lane >= x) incl += v;
+      }
+      int r = left - (incl - sum);  // still to take when this lane's bins begin
+      if (r > 0 && r <= sum) {
+        int i = 0;
+        while (r > c[i]) r -= c[i++];
+        s_digit = 255 - 8 * lane - i;
+        s_left = r;
+        s_count = c[i];
+      }
     }
     __syncthreads();
     pre |= (uint32_t)s_digit << shift;
     mask |= 255u << shift;
     left = s_left;
+    if (left == s_count) break;  // the whole bucket stays: no finer threshold needed
     __syncthreads();
   }
-  // Warp w compacts the contiguous slots [w * per, (w + 1) * per).
-  const int per = ((old + 31) / 32 + 31) / 32 * 32;
+  // Warp w compacts the contiguous slots [w * per, (w + 1) * per), a lane's
+  // four in order.
+  const int per = ((old + 31) / 32 + 127) / 128 * 128;
   const int t_lo = min(old, warp * per), t_hi = min(old, t_lo + per);
   __shared__ int s_gt[32], s_eq[32];
   int gt = 0, eq = 0;
-  for (int t = t_lo + lane; t - lane < t_hi; t += 32) {
-    const uint32_t k = t < t_hi && want > 0 ? key(t) : 0u;
-    const bool in = t < t_hi && want > 0;
-    gt += __popc(__ballot_sync(0xffffffffu, in && k > pre));
-    eq += __popc(__ballot_sync(0xffffffffu, in && k == pre));
+  for (int t = t_lo + 4 * lane; t < t_hi; t += 128) {
+    const uint4 k4 = key4(t);
+    const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      gt += t + i < t_hi && (k[i] & mask) > pre;
+      eq += t + i < t_hi && (k[i] & mask) == pre;
+    }
+  }
+#pragma unroll
+  for (int x = 16; x; x >>= 1) {
+    gt += __shfl_xor_sync(0xffffffffu, gt, x);
+    eq += __shfl_xor_sync(0xffffffffu, eq, x);
   }
   if (lane == 0) s_gt[warp] = gt, s_eq[warp] = eq;
   __syncthreads();
   int eq0 = 0, at = 0;  // equal keys and kept slots before this warp's
-  for (int w = 0; w < warp; ++w) {
-    at += s_gt[w] + min(s_eq[w], max(0, left - eq0));
-    eq0 += s_eq[w];
+  {
+    const int e = s_eq[lane];
+    int incl = e;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, x);
+      if (lane >= x) incl += v;
+    }
+    const int before = incl - e, take = s_gt[lane] + min(e, max(0, left - before));
+    int sum = lane < warp ? take : 0;
+#pragma unroll
+    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    at = sum;
+    eq0 = __shfl_sync(0xffffffffu, before, warp);
   }
-  for (int t = t_lo + lane; t - lane < t_hi; t += 32) {
-    const bool in = t < t_hi && want > 0;
-    const uint32_t k = in ? key(t) : 0u;
-    const unsigned below = (1u << lane) - 1u;
-    const unsigned me = __ballot_sync(0xffffffffu, in && k == pre);
-    const bool take = in && (k > pre || (k == pre && eq0 + __popc(me & below) < left));
-    const unsigned mt = __ballot_sync(0xffffffffu, take);
-    if (take) kept[at + __popc(mt & below)] = t;
-    at += __popc(mt);
-    eq0 += __popc(me);
+  for (int t0 = t_lo; t0 < t_hi; t0 += 128) {
+    const int t = t0 + 4 * lane;
+    uint32_t k[4] = {0, 0, 0, 0};
+    if (t < t_hi) {
+      const uint4 k4 = key4(t);
+      k[0] = k4.x, k[1] = k4.y, k[2] = k4.z, k[3] = k4.w;
+    }
+    int e = 0, m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e += t + i < t_hi && (k[i] & mask) == pre;
+    int incl = e;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, x);
+      if (lane >= x) incl += v;
+    }
+    int rank = eq0 + incl - e;
+    eq0 += __shfl_sync(0xffffffffu, incl, 31);
+    unsigned take = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (t + i >= t_hi) continue;
+      const uint32_t v = k[i] & mask;
+      if (v > pre || (v == pre && rank++ < left)) take |= 1u << i, ++m;
+    }
+    incl = m;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, x);
+      if (lane >= x) incl += v;
+    }
+    int out = at + incl - m;
+    at += __shfl_sync(0xffffffffu, incl, 31);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (take >> i & 1) kept[out++] = t + i;
   }
-  for (int i = tid; i < a.recent; i += kF8SelThreads) kept[want + i] = old + i;
 }
 
-// A warp per destination block, head and pool: 16 kept rows from anywhere in
-// the sequence, their common scale, their codes.  Bound by bytes.
+// Largest magnitude code of four, NaN (0x7f) counting as nothing: E4M3
+// magnitudes order as their bits do.
+__device__ __forceinline__ uint32_t f8_max4(uint32_t m, uint32_t c) {
+  c &= 0x7f7f7f7fu;
+  return __vmaxu4(m, c & ~__vcmpeq4(c, 0x7f7f7f7fu));
+}
+// Codes times 2^k, |k| <= 15, rounded to E4M3: exact in FP16 before that.
+__device__ __forceinline__ uint32_t f8_rescale4(uint32_t c, __half2 f) {
+  uint32_t out;
+  __half2 lo(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c & 0xffff), __NV_E4M3));
+  __half2 hi(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c >> 16), __NV_E4M3));
+  lo = __hmul2(lo, f);
+  hi = __hmul2(hi, f);
+  out = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(lo), __NV_SATFINITE, __NV_E4M3);
+  out |= (uint32_t)__nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(hi), __NV_SATFINITE, __NV_E4M3)
+         << 16;
+  return out;
+}
+
+// A warp per destination block and head: 16 kept rows of K and of V from
+// anywhere in the sequence, their common scales, their codes.  Bound by
+// bytes; the arithmetic stays on packed codes (magnitudes compared as bytes,
+// rows whose scale changes multiplied in FP16 pairs): on FP32 values it
+// took 82 us where the bytes of 16 x 4096 slots x 8 heads take 41.
 template <int D>
 __global__ void __launch_bounds__(128) f8_move_kernel(const __grid_constant__ F8EvictArgs a) {
   constexpr int NC = kF8Blk * D / 16 / 32;  // 16-byte chunks per lane
+  constexpr int LR = D / 16;                // lanes of a row
   const int lane = threadIdx.x & 31;
   const int item = blockIdx.x * 4 + (threadIdx.x >> 5);
   const int nkv = a.src.nkv, b = blockIdx.y;
-  const int kv = item & 1, h = (item >> 1) % nkv, blk = (item >> 1) / nkv;
+  const int h = item % nkv, blk = item / nkv;
   const int m = min(a.seqs[b].n, a.budget);
   const int j0 = blk * kF8Blk;
+  ptx::pdl_wait();
   if (j0 >= m) return;
   const int* kept = a.kept + ((long long)b * nkv + h) * a.budget + j0;
   const int ps = a.src.page_size, pd = a.dst.page_size;
+  const int rows = min(kF8Blk, m - j0);
+  const long long dhp = (long long)a.dst.bt[(long long)b * a.dst.max_pages + j0 / pd] * nkv + h;
   // lane r (< 16) holds where destination row r comes from
   long long src = 0;
-  float sscale = 0.f;
-  const int* bt = a.src.bt + (long long)b * a.src.max_pages;
-  const long long dhp = (long long)a.dst.bt[(long long)b * a.dst.max_pages + j0 / pd] * nkv + h;
-  if (lane < kF8Blk && j0 + lane < m) {
-    const int t = kept[lane];
-    const long long hp = (long long)bt[t / ps] * nkv + h;
-    src = hp * ps + t % ps;
-    sscale = (kv ? a.src.v_scale : a.src.k_scale)[hp * (ps / kF8Blk) + (t % ps) / kF8Blk];
-    if (kv == 0 && a.win) a.wout[dhp * pd + j0 % pd + lane] = a.win[src];
+  float ks = 0.f, vs = 0.f;
+  if (lane < rows) {
+    const int t = kept[lane], page = t / ps, sub = t - page * ps;
+    const long long hp = (long long)a.src.bt[(long long)b * a.src.max_pages + page] * nkv + h;
+    src = hp * ps + sub;
+    ks = a.src.k_scale[hp * (ps / kF8Blk) + sub / kF8Blk];
+    vs = a.src.v_scale[hp * (ps / kF8Blk) + sub / kF8Blk];
   }
-  const uint8_t* pool = kv ? a.src.v : a.src.k;
-  uint4 c[NC];
-  float sc[NC], amax = 0.f;
+  uint4 c[2][NC];
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
-    const int e = (lane + 32 * i) * 16, r = e / D;
-    const long long row = __shfl_sync(0xffffffffu, src, r);
-    sc[i] = __shfl_sync(0xffffffffu, sscale, r);
-    c[i] = make_uint4(0, 0, 0, 0);
-    if (j0 + r < m) c[i] = *reinterpret_cast<const uint4*>(pool + row * D + e % D);
-  }
-#pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
-    float x[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f8_decode4(w[j], sc[i], x);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) amax = fmaxf(amax, finite_abs(x[q]));
+    const int r = (lane + 32 * i) / LR;
+    const long long at = __shfl_sync(0xffffffffu, src, r) * D + (lane % LR) * 16;
+    c[0][i] = c[1][i] = make_uint4(0, 0, 0, 0);
+    if (r < rows) {
+      c[0][i] = *reinterpret_cast<const uint4*>(a.src.k + at);
+      c[1][i] = *reinterpret_cast<const uint4*>(a.src.v + at);
     }
   }
-  const float s = f8_block_scale(warp_max(amax)), inv = f8_inv_pow2(s);
-  uint8_t* out = (kv ? a.dst.v : a.dst.k) + (dhp * pd + j0 % pd) * D;
+  if (lane < rows) a.wout[dhp * pd + j0 % pd + lane] = a.win[src];
 #pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int e = (lane + 32 * i) * 16, r = e / D;
-    if (j0 + r >= m) continue;
-    uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
-    float x[4];
+  for (int kv = 0; kv < 2; ++kv) {
+    const float sc = kv ? vs : ks;  // lane r: row r's
+    float amax = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f8_decode4(w[j], sc[i], x);
-      w[j] = f8_encode4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+    for (int i = 0; i < NC; ++i) {
+      const uint4 w = c[kv][i];
+      uint32_t mx = f8_max4(f8_max4(f8_max4(f8_max4(0, w.x), w.y), w.z), w.w);
+      mx = max(max(mx & 255, mx >> 8 & 255), max(mx >> 16 & 255, mx >> 24));
+      const float v = __half2float(__half(__nv_cvt_fp8_to_halfraw((uint8_t)mx, __NV_E4M3)));
+      amax = fmaxf(amax, v * __shfl_sync(0xffffffffu, sc, (lane + 32 * i) / LR));
     }
-    *reinterpret_cast<uint4*>(out + e) = make_uint4(w[0], w[1], w[2], w[3]);
+    const float s = f8_block_scale(warp_max(amax));
+    // lane r: exponent of row r's factor
+    const int ex = (int)(__float_as_uint(sc) >> 23) - (int)(__float_as_uint(s) >> 23);
+    uint8_t* out = (kv ? a.dst.v : a.dst.k) + (dhp * pd + j0 % pd) * D;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int r = (lane + 32 * i) / LR;
+      const int k = __shfl_sync(0xffffffffu, ex, r);
+      if (r >= rows) continue;
+      uint32_t w[4] = {c[kv][i].x, c[kv][i].y, c[kv][i].z, c[kv][i].w};
+      if (k != 0) {
+        if (k >= -14 && k <= 15) {
+          const __half2 f = __half2half2(__ushort_as_half((unsigned short)((k + 15) << 10)));
+#pragma unroll
+          for (int q = 0; q < 4; ++q) w[q] = f8_rescale4(w[q], f);
+        } else {
+          const float f = f8_exp2i(max(-126, min(127, k)));
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
+            float x[4];
+            f8_decode4(w[q], f, x);
+            w[q] = f8_encode4(x[0], x[1], x[2], x[3]);
+          }
+        }
+      }
+      *reinterpret_cast<uint4*>(out + (lane + 32 * i) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (lane == 0)
+      (kv ? a.dst.v_scale : a.dst.k_scale)[dhp * (pd / kF8Blk) + (j0 % pd) / kF8Blk] = s;
   }
-  if (lane == 0)
-    (kv ? a.dst.v_scale : a.dst.k_scale)[dhp * (pd / kF8Blk) + (j0 % pd) / kF8Blk] = s;
 }
 
 }  // namespace molot
