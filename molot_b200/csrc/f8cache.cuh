@@ -439,10 +439,8 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
       const float ksc = __shfl_sync(0xffffffffu, ks_run, m & 31);
       const float vsc = __shfl_sync(0xffffffffu, vs_run, m & 31);
       const uint32_t src = ring + st_get * F::kBlk, vsrc = src + kF8Blk * D;
-      if (!s_abort && !ptx::mbar_wait_bounded(full + st_get, phase, a.timeout_ns)) {
-        s_abort = 1;
+      if (!ptx::mbar_wait_abort(full + st_get, phase, a.timeout_ns, &s_abort))
         atomicCAS(a.status, 0, 1);
-      }
       __syncwarp();
       if (++st_get == F::kStages) st_get = 0, phase ^= 1;
       // S^T: two chains, so that a product need not wait for the last one

@@ -75,13 +75,15 @@ struct PackedShape {
   // which would wait for tensor memory, fits the SM
   static constexpr int kSlots = D == 64 ? 8 : 4;
   static constexpr int kVSlots = kSlots / 2;
+  // kPoly of kPolyOf pairs of weights take the FMA pipe's exponential
+  static constexpr int kPoly = 0, kPolyOf = 4;
   static constexpr int kQ = 128 * D * 2;            // bytes of a Q tile
   static constexpr int kKV = BN * D * 2;            // bytes of a ring slot
   static constexpr int kBar = kTiles * kQ + kSlots * kKV;
   static constexpr int kSmem = kBar + 512 + 1024;   // + alignment
   static constexpr uint32_t kS = 0, kO = kBufs * BN;  // tensor-memory columns
   static constexpr int kSoft = 128 * kTiles;        // softmax threads
-  static constexpr int kThreads = kSoft + 128;
+  static constexpr int kThreads = kSoft + 256;
   static_assert(kO + kTiles * D <= 512, "tensor memory");
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -100,24 +102,39 @@ __host__ __device__ constexpr uint32_t idesc(bool bf, int n, bool mn) {
   return (1u << 4) | ((bf ? 1u : 0u) << 7) | ((bf ? 1u : 0u) << 10) | ((mn ? 1u : 0u) << 16) |
          ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, int acc) {
+// The products and commits below are issued by the whole warp with `go` set
+// in one lane: control stays uniform, so descriptors are computed in uniform
+// registers, where the instructions want them.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t p;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(acc)
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(p));
+  return p;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, int acc,
+                                       uint32_t go) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(acc), "r"(go)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, int acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, int acc,
+                                       uint32_t go) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(acc)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(acc), "r"(go)
       : "memory");
 }
-__device__ __forceinline__ void commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   ptx::smem_u32(bar))
-               : "memory");
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t go) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          ptx::smem_u32(bar)),
+      "r"(go)
+      : "memory");
 }
 __device__ __forceinline__ void fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -150,6 +167,13 @@ __device__ __forceinline__ void st32(uint32_t addr, const uint32_t* r) {
       PK_R8(r, 0), PK_R8(r, 8), PK_R8(r, 16), PK_R8(r, 24)
       : "memory");
 }
+__device__ __forceinline__ void st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15,%16};" ::"r"(addr),
+      PK_R8(r, 0), PK_R8(r, 8)
+      : "memory");
+}
 __device__ __forceinline__ void wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -171,6 +195,29 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   else
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+// 2^z on the FMA pipe, for z in [-126, 126]: z = n + r, |r| <= 1/2, 2^r by the
+// degree-4 polynomial of least relative error (2.6e-6; fitted with reweighted
+// least squares), n added to the exponent.
+__device__ __forceinline__ float2 exp2_poly(float2 z) {
+  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer
+  z.x = fmaxf(z.x, -126.f), z.y = fmaxf(z.y, -126.f);
+  const float2 t = __fadd2_rn(z, make_float2(kMagic, kMagic));
+  const float2 r = __fadd2_rn(z, __fmul2_rn(__fadd2_rn(t, make_float2(-kMagic, -kMagic)),
+                                            make_float2(-1.f, -1.f)));
+  float2 p = make_float2(0.009570102f, 0.009570102f);
+  p = __ffma2_rn(p, r, make_float2(0.05591786f, 0.05591786f));
+  p = __ffma2_rn(p, r, make_float2(0.24024744f, 0.24024744f));
+  p = __ffma2_rn(p, r, make_float2(0.6931218f, 0.6931218f));
+  p = __ffma2_rn(p, r, make_float2(0.9999993f, 0.9999993f));
+  p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
+  p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
+  return p;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 // Bits [lo, hi) of 32.
 __device__ __forceinline__ uint32_t bits(int lo, int hi) {
@@ -201,16 +248,17 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
   uint64_t* empty = bars + S::kSlots;     // [kSlots]
   uint64_t* s_full = empty + S::kSlots;   // [2]
   uint64_t* p_full = s_full + 2;          // [2]
-  uint64_t* o_full = p_full + 2;
+  uint64_t* p_half = p_full + 2;          // [2]
+  uint64_t* o_full = p_half + 2;
   uint64_t* q_full = o_full + 1;
   uint64_t* pv_done = q_full + 1;  // one row tile: P V of a key tile
-  uint64_t* v_ok = pv_done + 1;    // [kVSlots]
-  uint32_t* bad = reinterpret_cast<uint32_t*>(v_ok + S::kVSlots);  // [kVSlots][4] keys
+  uint64_t* kv_ok = pv_done + 1;   // [kVSlots] V_j looked over, K_(j + 1) there
+  uint32_t* bad = reinterpret_cast<uint32_t*>(kv_ok + S::kVSlots);  // [kVSlots][4] keys
   volatile uint32_t* tmem_sm = bad + 4 * S::kVSlots;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bad + 4 * S::kVSlots + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int kTmaWarp = S::kSoft / 32, kMmaWarp = kTmaWarp + 1;
+  constexpr int kTmaWarp = S::kSoft / 32, kMmaWarp = kTmaWarp + 1, kLookWarp = kTmaWarp + 4;
   const int g = blockIdx.x % a.nkv;
   const PackedItem it = a.items[blockIdx.x / a.nkv];
   // positions of the item's rows, and the key tiles they see
@@ -230,14 +278,12 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
            (t0 + BN - 1 <= pos0 && (a.window <= 0 || pos_last - t0 < a.window));
   };
   auto wait = [&](uint64_t* bar, uint32_t par, int code) {
-    if (*abort_flag) return;
-    if (!ptx::mbar_wait_bounded(bar, par, a.timeout_ns)) {
-      *abort_flag = 1;
-      atomicCAS(a.status, 0, code);
-    }
+    if (ptx::mbar_wait_abort(bar, par, a.timeout_ns, abort_flag)) return true;
+    atomicCAS(a.status, 0, code);
+    return false;
   };
 
-  if (tid == 0) {
+  if (tid == kTmaWarp * 32) {
     for (int i = 0; i < S::kSlots; ++i) {
       ptx::mbar_init(full + i, 1);
       ptx::mbar_init(empty + i, 1);
@@ -245,13 +291,25 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(s_full + i, 1);
       ptx::mbar_init(p_full + i, 128);
+      ptx::mbar_init(p_half + i, 128);
     }
     ptx::mbar_init(o_full, 1);
     ptx::mbar_init(q_full, 1);
     ptx::mbar_init(pv_done, 1);
-    for (int i = 0; i < S::kVSlots; ++i) ptx::mbar_init(v_ok + i, 64);
+    for (int i = 0; i < S::kVSlots; ++i) ptx::mbar_init(kv_ok + i, 128);
     *abort_flag = 0;
     ptx::fence_mbar_init();
+    // the first copies need not wait for the others
+    if (ntiles > 0) {
+      ptx::mbar_arrive_expect_tx(q_full, NT * a.G * a.BP * D * 2);
+      ptx::mbar_arrive_expect_tx(full, S::kKV);
+      for (int c = 0; c < D / 64; ++c) {
+        for (int i = 0; i < NT; ++i)
+          pk::tma3(smem + i * S::kQ + c * 128 * 128, &mq, c * 64, g * a.G,
+                   it.q0 + it.m0 + i * a.BP, q_full);
+        pk::tma3(kv + c * BN * 128, &mk, c * 64, g, it.k0 + tile_of(0) * BN, full);
+      }
+    }
   }
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -262,12 +320,13 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
   pk::fence_before();
   __syncthreads();
   pk::fence_after();
+  // All 512 columns: they start at 0, which the products take for granted
   const uint32_t tm = *tmem_sm;
 
   if (warp < kTmaWarp) {
     // ------------------------------------------------------------- softmax
-    // 384 threads x 168 registers: 256 x 224 + 128 x 56
-    if constexpr (NT == 2) ptx::setmaxnreg_inc<224>();
+    // 512 threads x 128 registers: 256 x 208 + 256 x 48
+    if constexpr (NT == 2) ptx::setmaxnreg_inc<208>();
     const int tile = warp >> 2;
     const int r = tid & 127;
     const uint32_t lane_base = tm + ((uint32_t)((warp & 3) * 32) << 16);
@@ -282,6 +341,17 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
     const float sl = a.scale * kLog2e;
     const float slope = kMode != kPlain && a.slopes && valid ? a.slopes[head] * kLog2e : 0.f;
     const float cap2 = a.cap * kLog2e, in = kMode == kCap ? a.scale / a.cap : 0.f;
+    // For |y| <= kCapPoly, y = x * in, cap2 * tanh(y) = x * P(y^2) with these
+    // coefficients (relative error 3e-8, fitted with reweighted least
+    // squares); beyond, cap2 - 2 cap2 / (e^(2y) + 1), whose end values are
+    // exact.  The polynomial alone serves a tile of smaller scores.
+    constexpr float kCapPoly = 0.75f;
+    const float ct[6] = {sl,
+                         -0.33332959f * sl,
+                         0.13325405f * sl,
+                         -0.053344406f * sl,
+                         0.019582849f * sl,
+                         -0.004716210f * sl};
     // kPlain: m and the scores are in units of raw products, sl brings them
     // to base 2; else they are base-2 already.
     const float unit = kMode == kPlain ? sl : 1.f;
@@ -298,30 +368,68 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
 #pragma unroll
       for (int c = 0; c < BN; c += 32) pk::wait_ld(s + c);
       const int t0 = tile_of(j) * BN;
-      if (kMode != kPlain) {
-        const float d0 = (float)(t0 - pos);
+      const bool edge = !whole(t0);
+      if (kMode == kCap) {
+        float am = 0.f;
 #pragma unroll
-        for (int i = 0; i < BN; ++i) {
-          float x = __uint_as_float(s[i]);
-          if (kMode == kCap) {
-            x = fmaf(-slope, fabsf(d0 + i), cap2 * tanhf(x * in));
-          } else {
-            x = fmaf(x, sl, -slope * fabsf(d0 + i));
+        for (int i = 0; i < BN; ++i) am = fmaxf(am, fabsf(__uint_as_float(s[i])));
+        if (__any_sync(0xffffffffu, !(am * fabsf(in) <= kCapPoly))) {
+#pragma unroll
+          for (int i = 0; i < BN; ++i) {
+            const float x = __uint_as_float(s[i]), y = x * in, y2 = y * y;
+            float q = ct[5];
+#pragma unroll
+            for (int k = 4; k >= 0; --k) q = fmaf(q, y2, ct[k]);
+            const float w = fmaf(-2.f * cap2, pk::rcp(ex2(y * (2.f * kLog2e)) + 1.f), cap2);
+            s[i] = __float_as_uint(fabsf(y) <= kCapPoly ? x * q : w);
           }
-          s[i] = __float_as_uint(x);
+        } else {
+#pragma unroll
+          for (int i = 0; i < BN; i += 2) {
+            const float2 x = make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+            const float2 y = __fmul2_rn(x, make_float2(in, in)), y2 = __fmul2_rn(y, y);
+            float2 q = make_float2(ct[5], ct[5]);
+#pragma unroll
+            for (int k = 4; k >= 0; --k) q = __ffma2_rn(q, y2, make_float2(ct[k], ct[k]));
+            q = __fmul2_rn(q, x);
+            s[i] = __float_as_uint(q.x), s[i + 1] = __float_as_uint(q.y);
+          }
         }
       }
-      if (!whole(t0)) {
-        // on a tile whose V was looked over: a row that sees a bad key is NaN
+      if (kMode == kBias || (kMode == kCap && a.slopes)) {
+        const float mul = kMode == kBias ? sl : 1.f, d0 = (float)(t0 - pos);
+        if (it.prefix == 0 || t0 + BN - 1 <= pos0) {
+          // no row sees keys beyond itself: -slope |pos - t| = slope (t - pos)
+          const float2 base = make_float2(slope * d0, slope * (d0 + 1.f));
+#pragma unroll
+          for (int i = 0; i < BN; i += 2) {
+            const float2 c =
+                __ffma2_rn(make_float2(slope, slope), make_float2((float)i, (float)i), base);
+            const float2 x =
+                __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])),
+                           make_float2(mul, mul), c);
+            s[i] = __float_as_uint(x.x), s[i + 1] = __float_as_uint(x.y);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < BN; ++i)
+            s[i] = __float_as_uint(
+                fmaf(__uint_as_float(s[i]), mul, -slope * fabsf(d0 + (float)i)));
+        }
+      }
+      if (edge) {
+        // V was looked over: a row that sees a bad key is NaN
         const int slot = j % S::kVSlots;
-        wait(v_ok + slot, (j / S::kVSlots) & 1, 2);
+        wait(kv_ok + slot, (j / S::kVSlots) & 1, 2);
 #pragma unroll
         for (int c = 0; c < BN; c += 32) {
           const uint32_t see =
               pk::bits(r_lo - t0 - c, r_hi - t0 - c) | pk::bits(0, r_pre - t0 - c);
+          if (!__all_sync(0xffffffffu, see == 0xffffffffu)) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!((see >> i) & 1)) s[c + i] = 0xff800000u;
+            for (int i = 0; i < 32; ++i)
+              if (!((see >> i) & 1)) s[c + i] = 0xff800000u;
+          }
           if (bad[slot * 4 + c / 32] & see) l = CUDART_NAN_F;
         }
       }
@@ -334,24 +442,26 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
         for (int k = 0; k < 4; ++k) mc4[k] = fmaxf(mc4[k], __uint_as_float(s[i + k]));
       const float mc = fmaxf(fmaxf(mc4[0], mc4[1]), fmaxf(mc4[2], mc4[3]));
       const bool raise = (mc - mx) * unit > 8.f || (mx == -CUDART_INF_F && mc > mx);
-      const bool resc = raise && mx != -CUDART_INF_F;
-      const float alpha = resc ? ex2((mx - mc) * unit) : 1.f;
-      if (raise) mx = mc;
-      l *= alpha;
-      if (__any_sync(0xffffffffu, resc)) {
-        if (NT == 1) {  // Q K of this tile was issued before P V of the last
-          wait(pv_done, (j - 1) & 1, 2);
-          __syncwarp();
-          pk::fence_after();
-        }
+      if (__any_sync(0xffffffffu, raise)) {
+        const bool resc = raise && mx != -CUDART_INF_F;
+        const float alpha = resc ? ex2((mx - mc) * unit) : 1.f;
+        if (raise) mx = mc;
+        l *= alpha;
+        if (__any_sync(0xffffffffu, resc)) {
+          if (NT == 1) {  // Q K of this tile was issued before P V of the last
+            wait(pv_done, (j - 1) & 1, 2);
+            __syncwarp();
+            pk::fence_after();
+          }
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          pk::ld32(o_col + c, o);
-          pk::wait_ld(o);
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            pk::ld32(o_col + c, o);
+            pk::wait_ld(o);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          pk::st32(o_col + c, o);
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            pk::st32(o_col + c, o);
+          }
         }
       }
       // (s - m) * unit, not s * unit - m * unit: the subtraction is exact near
@@ -359,24 +469,37 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
       const float neg = mx == -CUDART_INF_F ? 0.f : -mx;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < BN; c += 64) {
-        uint32_t p[32];
+      for (int c = 0; c < BN; c += BN / 2) {
+        uint32_t p[BN / 4];
+        auto weights = [&](auto poly) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float2 z = __fadd2_rn(make_float2(__uint_as_float(s[c + 2 * i]),
-                                            __uint_as_float(s[c + 2 * i + 1])),
-                                make_float2(neg, neg));
-          if (kMode == kPlain) z = __fmul2_rn(z, make_float2(unit, unit));
-          const float x = ex2(z.x), y = ex2(z.y);
-          sum[i & 1] = __fadd2_rn(sum[i & 1], make_float2(x, y));
-          p[i] = pk::pack2<T>(x, y);
-        }
-        pk::st32(s_col + c / 2, p);
+          for (int i = 0; i < BN / 4; ++i) {
+            float2 z = __fadd2_rn(make_float2(__uint_as_float(s[c + 2 * i]),
+                                              __uint_as_float(s[c + 2 * i + 1])),
+                                  make_float2(neg, neg));
+            if (kMode == kPlain) z = __fmul2_rn(z, make_float2(unit, unit));
+            if (decltype(poly)::value && i % S::kPolyOf < S::kPoly)
+              z = pk::exp2_poly(z);
+            else
+              z = make_float2(ex2(z.x), ex2(z.y));
+            sum[i & 1] = __fadd2_rn(sum[i & 1], z);
+            p[i] = pk::pack2<T>(z.x, z.y);
+          }
+        };
+        // exp2_poly has no weight of exactly 0 for masked keys
+        if (edge)
+          weights(std::false_type{});
+        else
+          weights(std::true_type{});
+        if (BN == 128)
+          pk::st32(s_col + c / 2, p);
+        else
+          pk::st16(s_col + c / 2, p);
+        pk::wait_st();
+        pk::fence_before();
+        ptx::mbar_arrive((c ? p_full : p_half) + buf);
       }
       l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-      pk::wait_st();
-      pk::fence_before();
-      ptx::mbar_arrive(p_full + buf);
     }
     // epilogue
     if (ntiles > 0) {
@@ -386,53 +509,66 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     const long long row = ((long long)it.q0 + m) * a.nq + head;
-    T* op = static_cast<T*>(a.o) + row * D;
-#pragma unroll 1
-    for (int c = 0; c < D; c += 32) {
-      uint32_t o[32];
+    // Rows go through shared memory (Q's, which no product reads any more),
+    // 16-byte pieces swizzled by row, so that stores cover whole rows.
+    unsigned char* rows = smem + tile * S::kQ + (warp & 3) * 32 * (D * 2);
+    constexpr int kPieces = D / 8;  // of a row
+#pragma unroll
+    for (int c = 0; c < D; c += 64) {
+      uint32_t o[64];
       if (ntiles > 0) {
         pk::ld32(o_col + c, o);
+        pk::ld32(o_col + c + 32, o + 32);
         pk::wait_ld(o);
-      }
-      if (valid) {
+        pk::wait_ld(o + 32);
+      } else {
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          uint32_t w[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            w[k] = ntiles > 0 ? pk::pack2<T>(__uint_as_float(o[i + 2 * k]) * inv,
-                                             __uint_as_float(o[i + 2 * k + 1]) * inv)
-                              : 0u;
-          *reinterpret_cast<uint4*>(op + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        for (int i = 0; i < 64; ++i) o[i] = 0;
       }
+#pragma unroll
+      for (int i = 0; i < 64; i += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          w[k] = pk::pack2<T>(__uint_as_float(o[i + 2 * k]) * inv,
+                              __uint_as_float(o[i + 2 * k + 1]) * inv);
+        const int piece = (c + i) / 8;
+        *reinterpret_cast<uint4*>(rows + lane * (D * 2) + ((piece ^ (lane & 7)) * 16)) =
+            make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    __syncwarp();
+    // where the warp's rows go (-1: nowhere), a lane each
+    const long long dst = valid ? row : -1;
+#pragma unroll 4
+    for (int i = lane; i < 32 * kPieces; i += 32) {
+      const int rr = i / kPieces, piece = i % kPieces;
+      const long long to = __shfl_sync(0xffffffffu, dst, rr);
+      const uint4 v =
+          *reinterpret_cast<const uint4*>(rows + rr * (D * 2) + ((piece ^ (rr & 7)) * 16));
+      if (to >= 0) reinterpret_cast<uint4*>(static_cast<T*>(a.o) + to * D)[piece] = v;
     }
     if (valid && a.lse)
       a.lse[row] = l == 0.f ? -CUDART_INF_F : (mx * unit + log2f(l)) * kLn2;
     pk::fence_before();
   } else {
-    if constexpr (NT == 2) ptx::setmaxnreg_dec<56>();
+    if constexpr (NT == 2) ptx::setmaxnreg_dec<48>();
     if (warp == kTmaWarp) {
       // ---------------------------------------------------------- copies
       if (lane == 0 && ntiles > 0) {
-        ptx::mbar_arrive_expect_tx(q_full, NT * a.G * a.BP * D * 2);
-        for (int i = 0; i < NT; ++i)
-          for (int c = 0; c < D / 64; ++c)
-            pk::tma3(smem + i * S::kQ + c * 128 * 128, &mq, c * 64, g * a.G,
-                     it.q0 + it.m0 + i * a.BP, q_full);
         const int n = 2 * ntiles;
-        int k = 0;
-        for (; k < n && !*abort_flag; ++k) {
+        int k = 1;  // K_0 is on its way
+        bool ok = true;
+        for (; k < n; ++k) {
           const int slot = k % S::kSlots;
-          if (k >= S::kSlots) wait(empty + slot, (k / S::kSlots - 1) & 1, 4);
-          if (*abort_flag) break;
+          if (k >= S::kSlots && !(ok = wait(empty + slot, (k / S::kSlots - 1) & 1, 4))) break;
           ptx::mbar_arrive_expect_tx(full + slot, S::kKV);
           for (int c = 0; c < D / 64; ++c)
             pk::tma3(kv + slot * S::kKV + c * BN * 128, k & 1 ? &mv : &mk, c * 64, g,
                      it.k0 + tile_of(k >> 1) * BN, full + slot);
         }
         // copies in flight end before the CTA does
-        if (*abort_flag) {
+        if (!ok) {
           ptx::mbar_wait_bounded(q_full, 0, a.timeout_ns);
           for (int i = max(0, k - S::kSlots); i < k; ++i)
             ptx::mbar_wait_bounded(full + i % S::kSlots, (i / S::kSlots) & 1, a.timeout_ns);
@@ -440,107 +576,108 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
       }
     } else if (warp == kMmaWarp) {
       // -------------------------------------------------------- products
-      if (lane == 0 && ntiles > 0) {
+      if (ntiles > 0) {
+        const uint32_t go = pk::elect_one();
         constexpr uint32_t id_s = pk::idesc(kBf, BN, false), id_o = pk::idesc(kBf, D, true);
-        const uint32_t q_addr = ptx::smem_u32(smem), kv_addr = ptx::smem_u32(kv);
-        auto qk = [&](int tile, int j) {  // S = Q K_j^T
-          const uint32_t q = q_addr + tile * S::kQ, k = kv_addr + (2 * j) % S::kSlots * S::kKV;
-          const uint32_t d = tm + S::kS + (NT == 2 ? tile : j & 1) * BN;
+        const uint64_t dq = pk::desc128(ptx::smem_u32(smem), 0, 1024);
+        const uint64_t dk = pk::desc128(ptx::smem_u32(kv), 0, 1024);
+        const uint64_t dv = pk::desc128(ptx::smem_u32(kv), BN * 128, 1024);
+        auto qk = [&](int tile, int buf, int slot) {  // S = Q K^T
+          const uint64_t q = dq + (uint32_t)(tile * (S::kQ >> 4));
+          const uint64_t k = dk + (uint32_t)(slot * (S::kKV >> 4));
 #pragma unroll
           for (int c = 0; c < D / 16; ++c)
-            pk::mma_ss(d, pk::desc128(q + (c >> 2) * 128 * 128 + (c & 3) * 32, 0, 1024),
-                       pk::desc128(k + (c >> 2) * BN * 128 + (c & 3) * 32, 0, 1024), id_s, c > 0);
+            pk::mma_ss(S::kS + buf * BN, q + ((c >> 2) * 128 * 128 + (c & 3) * 32 >> 4),
+                       k + ((c >> 2) * BN * 128 + (c & 3) * 32 >> 4), id_s, c > 0, go);
+          pk::commit(s_full + buf, go);
         };
-        auto pv = [&](int tile, int j) {  // O += P V_j
-          const uint32_t v = kv_addr + (2 * j + 1) % S::kSlots * S::kKV;
-          const uint32_t p = tm + S::kS + (NT == 2 ? tile : j & 1) * BN;
+        auto pv = [&](int tile, int buf, int slot, int half, bool first) {  // O += P V, half the keys
+          const uint64_t v = dv + (uint32_t)(slot * (S::kKV >> 4));
 #pragma unroll
-          for (int c = 0; c < BN / 16; ++c)
-            pk::mma_ts(tm + S::kO + tile * D, p + c * 8,
-                       pk::desc128(v + c * 2048, BN * 128, 1024), id_o, j > 0 || c > 0);
-        };
-        auto full_of = [&](int k) { wait(full + k % S::kSlots, (k / S::kSlots) & 1, 5); };
-        wait(q_full, 0, 6);
-        full_of(0);
-        pk::fence_after();
-        for (int i = 0; i < NT && !*abort_flag; ++i) {
-          qk(i, 0);
-          pk::commit(s_full + i);
-        }
-        if (!*abort_flag) pk::commit(empty);  // K_0's slot
-        for (int j = 0; j < ntiles; ++j) {
-          const bool next = j + 1 < ntiles;
-          if (next) full_of(2 * j + 2);
-          if (NT == 1 && next && !*abort_flag) {  // the other S buffer
-            pk::fence_after();
-            qk(0, j + 1);
-            pk::commit(s_full + ((j + 1) & 1));
+          for (int c = 0; c < BN / 32; ++c) {
+            const int x = half * (BN / 32) + c;
+            pk::mma_ts(S::kO + tile * D, S::kS + buf * BN + x * 8, v + (x * 2048 >> 4),
+                       id_o, !first || x > 0, go);
           }
-          full_of(2 * j + 1);
-          if (!whole(tile_of(j) * BN)) wait(v_ok + j % S::kVSlots, (j / S::kVSlots) & 1, 2);
+        };
+        int ks = 0, vs = 1;  // ring slots of K_(j + 1) (after its step) and V_j
+        uint32_t vp = 0;     // phase of V_j's slot
+        bool ok = wait(q_full, 0, 6) && wait(full, 0, 5);
+        if (ok) {
+          pk::fence_after();
+          for (int i = 0; i < NT; ++i) qk(i, i, 0);
+          pk::commit(empty, go);
+        }
+        for (int j = 0; ok && j < ntiles; ++j) {
+          const bool next = j + 1 < ntiles;
+          ks = ks + 2 >= S::kSlots ? ks + 2 - S::kSlots : ks + 2;
+          // V_j looked over, K_(j + 1) there
+          if (!(ok = wait(kv_ok + (vs >> 1), vp, 2))) break;
+          if (NT == 1 && next) {  // the other S buffer
+            pk::fence_after();
+            qk(0, (j + 1) & 1, ks);
+          }
+#pragma unroll
           for (int i = 0; i < NT; ++i) {
             const int buf = NT == 2 ? i : j & 1;
-            wait(p_full + buf, (NT == 2 ? j : j >> 1) & 1, 7);
-            if (*abort_flag) break;
+            const uint32_t par = (NT == 2 ? j : j >> 1) & 1;
+            if (!(ok = ok && wait(p_half + buf, par, 7))) break;
             pk::fence_after();
-            pv(i, j);
-            if (NT == 1) pk::commit(pv_done);
-            if (NT == 2 && next) {
-              qk(i, j + 1);
-              pk::commit(s_full + i);
-            }
+            pv(i, buf, vs, 0, j == 0);
+            if (!(ok = wait(p_full + buf, par, 7))) break;
+            pk::fence_after();
+            pv(i, buf, vs, 1, j == 0);
+            if (NT == 2 && next) qk(i, buf, ks);
           }
-          if (*abort_flag) break;
-          pk::commit(empty + (2 * j + 1) % S::kSlots);
-          if (next) pk::commit(empty + (2 * j + 2) % S::kSlots);
+          if (!ok) break;
+          if (NT == 1) pk::commit(pv_done, go);
+          pk::commit(empty + vs, go);
+          if (next) pk::commit(empty + ks, go);
+          vs += 2;
+          if (vs >= S::kSlots) vs -= S::kSlots, vp ^= 1;
         }
-        pk::commit(o_full);
+        pk::commit(o_full, go);
         // the products in flight end before tensor memory is freed
-        if (*abort_flag) ptx::mbar_wait_bounded(o_full, 0, a.timeout_ns);
+        if (!ok) ptx::mbar_wait_bounded(o_full, 0, a.timeout_ns);
       }
-    } else {
+    } else if (warp >= kLookWarp) {
       // ------------------------------------------------- V's masked rows
-      const int w = (warp - kMmaWarp - 1) * 32 + lane;  // keys w, w + 64
+      const int key = tid - kLookWarp * 32;
       for (int j = 0; j < ntiles; ++j) {
         const int k = 2 * j + 1, slot = k % S::kSlots, vs = j % S::kVSlots;
-        wait(full + slot, (k / S::kSlots) & 1, 8);
-        if (whole(tile_of(j) * BN)) {
-          ptx::mbar_arrive(v_ok + vs);
-          continue;
-        }
-        bool any_fix = false;
-        for (int key = w; key < BN; key += 64) {
+        if (!wait(full + slot, (k / S::kSlots) & 1, 8)) break;
+        if (j + 1 < ntiles && !wait(full + (k + 1) % S::kSlots, ((k + 1) / S::kSlots) & 1, 8)) break;
+        if (!whole(tile_of(j) * BN)) {
           bool found = false;
-          if (!*abort_flag) {
-            for (int c = 0; c < D / 64; ++c) {
+          if (key < BN) {
+            // 16-byte pieces of the row, in whatever order the swizzle put them
+            unsigned char* row = kv + slot * S::kKV + key * 128;
+            constexpr uint32_t e = kBf ? 0x7f807f80u : 0x7c007c00u, one = kBf ? 0x00800080u : 0x04000400u;
+#pragma unroll 1
+            for (int i = 0; i < D / 8; i += 4) {
+              unsigned char* at = row + (i >> 3) * BN * 128 + (i & 4) * 16;
+              uint4 x[4];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                // 16-byte pieces of the row, in whatever order the swizzle put them
-                uint4* p = reinterpret_cast<uint4*>(kv + slot * S::kKV + c * BN * 128 + key * 128 +
-                                                    i * 16);
-                uint4 x = *p;
-                uint32_t* xw = &x.x;
-                bool hit = false;
-                constexpr uint32_t e = kBf ? 0x7f80u : 0x7c00u;
+              for (int q = 0; q < 4; ++q) x[q] = *reinterpret_cast<const uint4*>(at + q * 16);
+              // an exponent of all ones carries into the bit above it
+              uint32_t hit = 0;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  const bool b0 = (xw[q] & e) == e, b1 = (xw[q] & (e << 16)) == (e << 16);
-                  if (b0) xw[q] &= 0xffff0000u;
-                  if (b1) xw[q] &= 0x0000ffffu;
-                  hit |= b0 || b1;
-                }
-                if (hit) *p = x;
-                found |= hit;
-              }
+              for (int q = 0; q < 4; ++q)
+                hit |= ((x[q].x & e) + one) | ((x[q].y & e) + one) | ((x[q].z & e) + one) |
+                       ((x[q].w & e) + one);
+              if (!(hit & 0x80008000u)) continue;
+              found = true;
+              unsigned short* v = reinterpret_cast<unsigned short*>(at);
+              for (int q = 0; q < 32; ++q)
+                if ((v[q] & (e & 0xffff)) == (e & 0xffff)) v[q] = 0;
             }
           }
           const uint32_t word = __ballot_sync(0xffffffffu, found);
-          if (lane == 0) bad[vs * 4 + key / 32] = word;
-          any_fix |= found;
+          if (lane == 0 && key < BN) bad[vs * 4 + key / 32] = word;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
         }
-        if (any_fix) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        ptx::mbar_arrive(v_ok + vs);
+        ptx::mbar_arrive(kv_ok + vs);
       }
     }
   }

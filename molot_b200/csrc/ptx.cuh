@@ -62,6 +62,26 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   return true;
 }
 
+// The same with an abort flag in shared memory, raised by whoever gave up
+// first, that ends it too; nothing but the first try is on the path of a wait
+// that is over already.  (A try with a longer hint to the barrier unit cost 90
+// cycles more on that path; a spin without the timer's pause took issue slots
+// from the warps it waited for.)
+__device__ __forceinline__ bool mbar_wait_abort(uint64_t* bar, uint32_t parity, uint64_t limit_ns,
+                                                volatile int* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort_flag) return false;
+    if (globaltimer_ns() - t0 > limit_ns) {
+      *abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
 // L2 policy for data streamed exactly once (the KV rows).
 __device__ __forceinline__ uint64_t policy_evict_first() {
   uint64_t pol;
