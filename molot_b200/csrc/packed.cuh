@@ -14,26 +14,38 @@
 // in shared memory, brought by TMA with the 128-byte swizzle);  the row
 // tile's warpgroup reads its rows of S (a thread per row, so maxima and sums
 // never leave the thread), applies cap, bias and mask, and writes
-// P = 2^(x - m) in the operands' type over S's columns;  O_s += P V_j with P
-// from tensor memory and V as an MN-major operand, straight as TMA brought it.
-// m is raised, and O rescaled, only when a score passes it by 2^8: the
-// weights stay below 2^8, which costs nothing in BF16 and stays far inside
-// FP16's range.  P's rounding to 16 bits is what the tensor cores take; the
-// sum l is taken of the weights before it, in FP32.
+// P = 2^(x - m) in the operands' type over S's columns, in two halves;
+// O_s += P V_j with P from tensor memory and V as an MN-major operand,
+// straight as TMA brought it.  m is raised, and O rescaled, only when a score
+// passes it by 2^8: the weights stay below 2^8, which costs nothing in BF16
+// and stays far inside FP16's range.  P's rounding to 16 bits is what the
+// tensor cores take; the sum l is taken of the weights before it, in FP32.
 //
-// The issuing thread orders  PV_s(j), QK_s(j + 1)  for s = 0, 1, so one row
+// The issuing warp orders  PV_s(j), QK_s(j + 1)  for s = 0, 1, so one row
 // tile's products run while the other's softmax does, and the commit of
-// QK_s(j + 1) also tells that PV_s(j) is done: O and S may be touched.
+// QK_s(j + 1) also tells that PV_s(j) is done: O and S may be touched.  At
+// d = 256 there is one row tile and S has two buffers, and QK(j + 1) goes
+// ahead of PV(j).
 //
 // Masked keys.  Scores are replaced, so K may hold anything there.  V
 // multiplies weights of zero, and 0 * NaN is NaN, so on key tiles that some
-// row does not see entirely two warps look V over in shared memory, put
+// row does not see entirely four warps look V over in shared memory, put
 // zeros in the place of infinities and NaN, and name the keys; a row that
 // does see such a key becomes NaN.
 //
 // Warps: 0-3 (4-7) softmax of row tile 0 (1), epilogue; then one that issues
-// TMA copies, one that issues MMAs, two that look over V.  Every wait is
-// bounded; one that runs out records a status code and ends the CTA.
+// TMA copies, one that issues MMAs, two idle, four that look over V.  Every
+// wait is bounded; one that runs out records a status code and ends the CTA.
+//
+// Measured (16384 causal rows, 32 heads of 128 on 8, BF16): 1.74 ms, 1265
+// TFLOP/s, for a pass alone, 2.01 ms, 1090, back to back under the power
+// limit, where plain BF16 GEMMs run at 1640 and 1366.  Of the 3500 cycles a key
+// tile takes for both row tiles, the tensor pipe is busy 2048; a row tile's
+// chain is 110 reading S, 550 to the maximum, 1500 exponentials (1024 of the
+// MUFU), 230 storing P, 1050 for PV and QK.  Not kept: part of the
+// exponentials as polynomials on the FMA pipe (1.5 % faster alone, 1 % slower
+// back to back); two threads a row (the registers that a thread then has
+// spill); one row tile and two CTAs an SM (5 % slower: K and V come twice).
 #pragma once
 
 #include <cuda.h>
@@ -75,8 +87,6 @@ struct PackedShape {
   // which would wait for tensor memory, fits the SM
   static constexpr int kSlots = D == 64 ? 8 : 4;
   static constexpr int kVSlots = kSlots / 2;
-  // kPoly of kPolyOf pairs of weights take the FMA pipe's exponential
-  static constexpr int kPoly = 0, kPolyOf = 4;
   static constexpr int kQ = 128 * D * 2;            // bytes of a Q tile
   static constexpr int kKV = BN * D * 2;            // bytes of a ring slot
   static constexpr int kBar = kTiles * kQ + kSlots * kKV;
@@ -196,24 +206,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// 2^z on the FMA pipe, for z in [-126, 126]: z = n + r, |r| <= 1/2, 2^r by the
-// degree-4 polynomial of least relative error (2.6e-6; fitted with reweighted
-// least squares), n added to the exponent.
-__device__ __forceinline__ float2 exp2_poly(float2 z) {
-  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer
-  z.x = fmaxf(z.x, -126.f), z.y = fmaxf(z.y, -126.f);
-  const float2 t = __fadd2_rn(z, make_float2(kMagic, kMagic));
-  const float2 r = __fadd2_rn(z, __fmul2_rn(__fadd2_rn(t, make_float2(-kMagic, -kMagic)),
-                                            make_float2(-1.f, -1.f)));
-  float2 p = make_float2(0.009570102f, 0.009570102f);
-  p = __ffma2_rn(p, r, make_float2(0.05591786f, 0.05591786f));
-  p = __ffma2_rn(p, r, make_float2(0.24024744f, 0.24024744f));
-  p = __ffma2_rn(p, r, make_float2(0.6931218f, 0.6931218f));
-  p = __ffma2_rn(p, r, make_float2(0.9999993f, 0.9999993f));
-  p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
-  p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
-  return p;
-}
 __device__ __forceinline__ float rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -325,8 +317,8 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
 
   if (warp < kTmaWarp) {
     // ------------------------------------------------------------- softmax
-    // 512 threads x 128 registers: 256 x 208 + 256 x 48
-    if constexpr (NT == 2) ptx::setmaxnreg_inc<208>();
+    // 512 threads x 128 registers: 256 x 200 + 256 x 56
+    if constexpr (NT == 2) ptx::setmaxnreg_inc<200>();
     const int tile = warp >> 2;
     const int r = tid & 127;
     const uint32_t lane_base = tm + ((uint32_t)((warp & 3) * 32) << 16);
@@ -400,15 +392,20 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
         const float mul = kMode == kBias ? sl : 1.f, d0 = (float)(t0 - pos);
         if (it.prefix == 0 || t0 + BN - 1 <= pos0) {
           // no row sees keys beyond itself: -slope |pos - t| = slope (t - pos)
-          const float2 base = make_float2(slope * d0, slope * (d0 + 1.f));
+          float2 off[4];
 #pragma unroll
-          for (int i = 0; i < BN; i += 2) {
-            const float2 c =
-                __ffma2_rn(make_float2(slope, slope), make_float2((float)i, (float)i), base);
-            const float2 x =
-                __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])),
-                           make_float2(mul, mul), c);
-            s[i] = __float_as_uint(x.x), s[i + 1] = __float_as_uint(x.y);
+          for (int k = 0; k < 4; ++k) off[k] = make_float2(slope * (2 * k), slope * (2 * k + 1));
+#pragma unroll
+          for (int i = 0; i < BN; i += 8) {
+            const float base = slope * (d0 + (float)i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int c = i + 2 * k;
+              const float2 x =
+                  __ffma2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])),
+                             make_float2(mul, mul), __fadd2_rn(off[k], make_float2(base, base)));
+              s[c] = __float_as_uint(x.x), s[c + 1] = __float_as_uint(x.y);
+            }
           }
         } else {
 #pragma unroll
@@ -433,13 +430,13 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
           if (bad[slot * 4 + c / 32] & see) l = CUDART_NAN_F;
         }
       }
-      float mc4[4];
+      float mc4[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) mc4[k] = __uint_as_float(s[k]);
+      for (int i = 0; i < BN; i += 8)
 #pragma unroll
-      for (int i = 4; i < BN; i += 4)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) mc4[k] = fmaxf(mc4[k], __uint_as_float(s[i + k]));
+        for (int k = 0; k < 4; ++k)
+          mc4[k] = fmaxf(fmaxf(mc4[k], __uint_as_float(s[i + 2 * k])),
+                         __uint_as_float(s[i + 2 * k + 1]));
       const float mc = fmaxf(fmaxf(mc4[0], mc4[1]), fmaxf(mc4[2], mc4[3]));
       const bool raise = (mc - mx) * unit > 8.f || (mx == -CUDART_INF_F && mc > mx);
       if (__any_sync(0xffffffffu, raise)) {
@@ -471,26 +468,16 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
 #pragma unroll
       for (int c = 0; c < BN; c += BN / 2) {
         uint32_t p[BN / 4];
-        auto weights = [&](auto poly) {
 #pragma unroll
-          for (int i = 0; i < BN / 4; ++i) {
-            float2 z = __fadd2_rn(make_float2(__uint_as_float(s[c + 2 * i]),
-                                              __uint_as_float(s[c + 2 * i + 1])),
-                                  make_float2(neg, neg));
-            if (kMode == kPlain) z = __fmul2_rn(z, make_float2(unit, unit));
-            if (decltype(poly)::value && i % S::kPolyOf < S::kPoly)
-              z = pk::exp2_poly(z);
-            else
-              z = make_float2(ex2(z.x), ex2(z.y));
-            sum[i & 1] = __fadd2_rn(sum[i & 1], z);
-            p[i] = pk::pack2<T>(z.x, z.y);
-          }
-        };
-        // exp2_poly has no weight of exactly 0 for masked keys
-        if (edge)
-          weights(std::false_type{});
-        else
-          weights(std::true_type{});
+        for (int i = 0; i < BN / 4; ++i) {
+          float2 z = __fadd2_rn(make_float2(__uint_as_float(s[c + 2 * i]),
+                                            __uint_as_float(s[c + 2 * i + 1])),
+                                make_float2(neg, neg));
+          if (kMode == kPlain) z = __fmul2_rn(z, make_float2(unit, unit));
+          z = make_float2(ex2(z.x), ex2(z.y));
+          sum[i & 1] = __fadd2_rn(sum[i & 1], z);
+          p[i] = pk::pack2<T>(z.x, z.y);
+        }
         if (BN == 128)
           pk::st32(s_col + c / 2, p);
         else
@@ -513,27 +500,23 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
     // 16-byte pieces swizzled by row, so that stores cover whole rows.
     unsigned char* rows = smem + tile * S::kQ + (warp & 3) * 32 * (D * 2);
     constexpr int kPieces = D / 8;  // of a row
-#pragma unroll
-    for (int c = 0; c < D; c += 64) {
-      uint32_t o[64];
+    // (compact loops: code that runs once per CTA is fetched cold)
+#pragma unroll 1
+    for (int c = 0; c < D; c += 32) {
+      uint32_t o[32];
       if (ntiles > 0) {
         pk::ld32(o_col + c, o);
-        pk::ld32(o_col + c + 32, o + 32);
         pk::wait_ld(o);
-        pk::wait_ld(o + 32);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 64; ++i) o[i] = 0;
       }
 #pragma unroll
-      for (int i = 0; i < 64; i += 8) {
+      for (int i = 0; i < 32; i += 8) {
         uint32_t w[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          w[k] = pk::pack2<T>(__uint_as_float(o[i + 2 * k]) * inv,
-                              __uint_as_float(o[i + 2 * k + 1]) * inv);
-        const int piece = (c + i) / 8;
-        *reinterpret_cast<uint4*>(rows + lane * (D * 2) + ((piece ^ (lane & 7)) * 16)) =
+          w[k] = ntiles > 0 ? pk::pack2<T>(__uint_as_float(o[i + 2 * k]) * inv,
+                                           __uint_as_float(o[i + 2 * k + 1]) * inv)
+                            : 0u;
+        *reinterpret_cast<uint4*>(rows + lane * (D * 2) + (((c + i) / 8 ^ (lane & 7)) * 16)) =
             make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
@@ -541,8 +524,8 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
     // where the warp's rows go (-1: nowhere), a lane each
     const long long dst = valid ? row : -1;
 #pragma unroll 4
-    for (int i = lane; i < 32 * kPieces; i += 32) {
-      const int rr = i / kPieces, piece = i % kPieces;
+    for (int k = 0; k < kPieces; ++k) {
+      const int i = lane + 32 * k, rr = i / kPieces, piece = i % kPieces;
       const long long to = __shfl_sync(0xffffffffu, dst, rr);
       const uint4 v =
           *reinterpret_cast<const uint4*>(rows + rr * (D * 2) + ((piece ^ (rr & 7)) * 16));
@@ -552,7 +535,7 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
       a.lse[row] = l == 0.f ? -CUDART_INF_F : (mx * unit + log2f(l)) * kLn2;
     pk::fence_before();
   } else {
-    if constexpr (NT == 2) ptx::setmaxnreg_dec<48>();
+    if constexpr (NT == 2) ptx::setmaxnreg_dec<56>();
     if (warp == kTmaWarp) {
       // ---------------------------------------------------------- copies
       if (lane == 0 && ntiles > 0) {
