@@ -189,6 +189,19 @@ class Pager {
   void layer_pools(int layer, float** k_pool, float** v_pool) {
     check(molot_pager_layer_pools(h_, layer, k_pool, v_pool));
   }
+  // One layer of MOLOT_KV_F8B pools with a batch's device block table.
+  molot_f8b_layer f8_layer(int layer, const int* block_table, int page_size) {
+    float *k, *v;
+    molot_f8b_layer l = {};
+    check(molot_pager_layer_pools(h_, layer, &k, &v));
+    check(molot_pager_layer_blocks(h_, layer, &l.k_scale, &l.v_scale, &l.weight));
+    l.k = k;
+    l.v = v;
+    l.block_table = block_table;
+    l.max_pages = max_pages_;
+    l.page_size = page_size;
+    return l;
+  }
 
  private:
   molot_pager* h_ = nullptr;
@@ -233,6 +246,79 @@ class PagedPlan {
 
  private:
   molot_paged_plan* h_ = nullptr;
+};
+
+// Batch of one step over 8-bit block-scaled pools (molot_f8b_*): build once
+// per step, then write and decode per layer; evict moves the slots to keep.
+class F8Plan {
+ public:
+  F8Plan() { check(molot_f8b_plan_create(&h_)); }
+  ~F8Plan() { molot_f8b_plan_destroy(h_); }
+  F8Plan(const F8Plan&) = delete;
+  F8Plan& operator=(const F8Plan&) = delete;
+
+  // Host arrays of B; null: one new row each, start 0, no prefix.
+  void build(int B, int nq, int nkv, int d, const int* seq_lens, const int* new_lens = nullptr,
+             const int* starts = nullptr, const int* prefix = nullptr, int window = 0,
+             void* stream = nullptr) {
+    check(molot_f8b_plan_build(h_, B, nq, nkv, d, seq_lens, new_lens, starts, prefix, window,
+                               stream));
+    q_row_ = (long long)nq * d;
+    kv_row_ = (long long)nkv * d;
+  }
+  // Rows [new rows][nkv][d], contiguous (stride 0) or that many elements apart.
+  void write(const molot_f8b_layer& layer, const void* k, const void* v, int act_dtype,
+             long long k_stride = 0, long long v_stride = 0, void* stream = nullptr) {
+    check(molot_f8b_write(h_, &layer, k, v, act_dtype, k_stride ? k_stride : kv_row_,
+                          v_stride ? v_stride : kv_row_, stream));
+  }
+  void decode(const molot_f8b_layer& layer, const void* q, void* o, int act_dtype, float scale,
+              float softcap = 0.f, const float* slopes = nullptr, float* lse = nullptr,
+              float* weight_out = nullptr, long long q_stride = 0, void* stream = nullptr) {
+    check(molot_f8b_decode(h_, &layer, q, o, lse, act_dtype, q_stride ? q_stride : q_row_, scale,
+                           softcap, slopes, weight_out, stream));
+  }
+  void evict(const molot_f8b_layer& src, const molot_f8b_layer& dst, int budget, int recent,
+             int* kept, void* stream = nullptr) {
+    check(molot_f8b_evict(h_, &src, &dst, budget, recent, kept, stream));
+  }
+  // Synchronise and surface device-side wait timeouts.
+  void sync(void* stream = nullptr) { check(molot_f8b_check(h_, stream)); }
+
+ private:
+  molot_f8b_plan* h_ = nullptr;
+  long long q_row_ = 0, kv_row_ = 0;
+};
+
+// Prefill attention over packed documents (molot_packed_*).
+class PackedPlan {
+ public:
+  PackedPlan() { check(molot_packed_plan_create(&h_)); }
+  ~PackedPlan() { molot_packed_plan_destroy(h_); }
+  PackedPlan(const PackedPlan&) = delete;
+  PackedPlan& operator=(const PackedPlan&) = delete;
+
+  void build(int ndocs, int nq, int nkv, int d, const int* q_lens, const int* k_lens = nullptr,
+             const int* prefix = nullptr, int window = 0, void* stream = nullptr) {
+    check(molot_packed_plan_build(h_, ndocs, nq, nkv, d, q_lens, k_lens, prefix, window, stream));
+    q_row_ = (long long)nq * d;
+    kv_row_ = (long long)nkv * d;
+  }
+  // Strides in elements between rows, 0: contiguous.
+  void attend(const void* q, const void* k, const void* v, void* o, int act_dtype, float scale,
+              float softcap = 0.f, const float* slopes = nullptr, float* lse = nullptr,
+              long long q_stride = 0, long long k_stride = 0, long long v_stride = 0,
+              void* stream = nullptr) {
+    check(molot_packed_attend(h_, q, k, v, o, lse, act_dtype, q_stride ? q_stride : q_row_,
+                              k_stride ? k_stride : kv_row_, v_stride ? v_stride : kv_row_, scale,
+                              softcap, slopes, stream));
+  }
+  // Synchronise and surface device-side wait timeouts.
+  void sync(void* stream = nullptr) { check(molot_packed_check(h_, stream)); }
+
+ private:
+  molot_packed_plan* h_ = nullptr;
+  long long q_row_ = 0, kv_row_ = 0;
 };
 
 // Peer-gather group for kv-head sharding over the GPUs of one node
