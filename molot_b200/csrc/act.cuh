@@ -92,10 +92,4 @@ __device__ __forceinline__ float ex2(float x) {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// Score q.k * scale -> base-2 logit: cap, distance bias (dist = newest - slot).
-__device__ __forceinline__ float score_logit(float s, float cap, float slope, float dist) {
-  if (cap > 0.f) s = cap * tanhf(s / cap);
-  return (s - slope * dist) * kLog2e;
-}
-
 }  // namespace molot

@@ -194,8 +194,8 @@ __global__ void __launch_bounds__(128) f8_write_kernel(const __grid_constant__ F
 // its matrix operands.  Blocks come by TMA into a ring of the warp's own in
 // shared memory, swizzled so that those loads touch every bank once.
 //
-// Softmax in base 2 with one reference M per head, raised only when a
-// score passes it by 2^8.  What must not overflow FP16 is the weight times
+// Softmax in base 2 with one reference M per head, a whole number, raised only
+// when a score passes it by 2^8.  What must not overflow FP16 is the weight times
 // the scale 2^ev of the block's V, so M follows s + ev: P = 2^(s - M + 6 + ev)
 // <= 2^14 multiplies the codes, while l adds 2^(s - M + 38), which stays
 // within FP32 for every ev in [-64, 120].  O = sum(P * code) * 2^32 / l.
@@ -423,11 +423,13 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
     uint2 qh[KS];
 #pragma unroll
     for (int j = 0; j < KS; ++j) qh[j] = reinterpret_cast<const uint2*>(qs)[j * 32 + lane];
-    const float sc0 = a.scale * qinv[2 * t4], sc1 = a.scale * qinv[2 * t4 + 1];
+    // base-2 scores but for the cap, which comes before
+    const float unit = a.cap > 0.f ? a.scale : a.scale * kLog2e, cap2 = a.cap * kLog2e;
+    const float sc0 = unit * qinv[2 * t4], sc1 = unit * qinv[2 * t4 + 1];
     float slope0 = 0.f, slope1 = 0.f;
     if (a.slopes) {
-      if (2 * t4 < nh) slope0 = a.slopes[head0 + 2 * t4];
-      if (2 * t4 + 1 < nh) slope1 = a.slopes[head0 + 2 * t4 + 1];
+      if (2 * t4 < nh) slope0 = a.slopes[head0 + 2 * t4] * kLog2e;
+      if (2 * t4 + 1 < nh) slope1 = a.slopes[head0 + 2 * t4 + 1] * kLog2e;
     }
 
     float o[KS][4], m0 = -CUDART_INF_F, m1 = -CUDART_INF_F, l0 = 0.f, l1 = 0.f;
@@ -476,12 +478,14 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
         for (int r = 0; r < 4; ++r) z[r] = (s[0][r] + s[1][r]) * (r & 1 ? c1 : c0);
         if (a.cap > 0.f) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) z[r] = a.cap * tanhf(z[r] / a.cap);
+          for (int r = 0; r < 4; ++r) z[r] = cap2 * tanhf(z[r] / a.cap);
         }
-        const float dist = (float)(sq.n - 1 - (blk_t + g));
+        if (a.slopes) {
+          const float dist = (float)(sq.n - 1 - (blk_t + g));
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          z[r] = (z[r] - (r & 1 ? slope1 : slope0) * (dist - (r >> 1) * 8)) * kLog2e;
+          for (int r = 0; r < 4; ++r)
+            z[r] = fmaf(-(r & 1 ? slope1 : slope0), dist - (r >> 1) * 8, z[r]);
+        }
       }
       const bool edge = blk_t < sq.first || blk_t + kF8Blk > sq.n ||
                         (blk_t < sq.lo && blk_t + kF8Blk > sq.sink_end);
@@ -515,8 +519,8 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
           n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, k));
           n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, k));
         }
-        n0 = fmaxf(n0, m0);
-        n1 = fmaxf(n1, m1);
+        n0 = fmaxf(ceilf(n0), m0);
+        n1 = fmaxf(ceilf(n1), m1);
         const float f0 = n0 == m0 ? 1.f : ex2(m0 - n0), f1 = n1 == m1 ? 1.f : ex2(m1 - n1);
         m0 = n0, m1 = n1;
         l0 *= f0, l1 *= f1;
@@ -526,18 +530,18 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
           o[k][1] *= f1, o[k][3] *= f1;
         }
       }
-      // (no score yet: -inf + 0, a weight of 0)
-      const float r0 = m0 == -CUDART_INF_F ? 0.f : 38.f - m0;
-      const float r1 = m1 == -CUDART_INF_F ? 0.f : 38.f - m1;
-      const float up = vsc * 0x1p-32f;  // 2^(ev - 32)
+      // M and ev are whole numbers, so m - ev is exact, and so is the
+      // subtraction near the maximum (no score yet: -inf - 0, a weight of 0)
+      const float r0 = m0 == -CUDART_INF_F ? 0.f : m0 - ev;
+      const float r1 = m1 == -CUDART_INF_F ? 0.f : m1 - ev;
+      const float up = f8_inv_pow2(vsc) * 0x1p38f;  // 2^(38 - ev)
       float p[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        p[r] = ex2(z[r] + (r & 1 ? r1 : r0));
-      l0 += p[0] + p[2];
-      l1 += p[1] + p[3];
+      for (int r = 0; r < 4; ++r) p[r] = ex2(z[r] - (r & 1 ? r1 : r0));
+      l0 = fmaf(p[0] + p[2], up, l0);
+      l1 = fmaf(p[1] + p[3], up, l1);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) p[r] *= up;
+      for (int r = 0; r < 4; ++r) p[r] *= 64.f;
       const uint32_t h0 = pack_h2(p[0], p[1]), h1 = pack_h2(p[2], p[3]);
       const uint32_t b0 = movmatrix_trans(h0), b1 = movmatrix_trans(h1);
       uint32_t e0 = 0, e1 = 0;
@@ -957,17 +961,19 @@ __global__ void __launch_bounds__(kF8SelThreads) f8_select_kernel(const __grid_c
           atomicAdd(&hist[warp % kF8SelHists][(k[i] >> shift) & 255], 1);
     }
     __syncthreads();
+    if (tid < 256) {
+      int c = 0;
+#pragma unroll
+      for (int k = 0; k < kF8SelHists; ++k) c += hist[k][tid];
+      hist[0][tid] = c;  // (no other thread reads this column)
+    }
+    __syncthreads();
     if (warp == 0) {
       // lane l: bins 255 - 8 l down to 248 - 8 l; the digit is where the
       // count from the top reaches `left`
       int c[8], sum = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        c[i] = 0;
-#pragma unroll
-        for (int k = 0; k < kF8SelHists; ++k) c[i] += hist[k][255 - 8 * lane - i];
-        sum += c[i];
-      }
+      for (int i = 0; i < 8; ++i) sum += c[i] = hist[0][255 - 8 * lane - i];
       int incl = sum;
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) {
