@@ -91,22 +91,23 @@ struct molot_f8b_plan {
   int device = -1;
   bool built = false;
   int B = 0, nq = 0, nkv = 0, d = 0;
-  int max_len = 0, max_end = 0;  // longest sequence
+  int max_len = 0;               // longest sequence
   int rows = 0, touched = 0;     // new rows, blocks they touch
   long long visits = 0;          // block visits of a decode (per kv head)
   int* h_buf = nullptr;          // pinned staging
+  size_t h_cap = 0;              // ints
+  // One allocation: the uploaded plan, tickets (zero between launches), records
+  unsigned char* mem = nullptr;
   int* d_buf = nullptr;
-  size_t h_cap = 0, d_cap = 0;  // ints
+  int* tickets = nullptr;
+  float* rec = nullptr;
+  size_t d_cap = 0, tickets_cap = 0, rec_cap = 0;  // ints, ints, floats
   cudaEvent_t uploaded = nullptr;
   int grid = 0;     // decode CTAs
   int cluster = 0;  // of so many CTAs
   size_t o_ctas = 0, o_prefix = 0, o_n0 = 0, o_len = 0, o_row = 0, o_blk = 0;  // F8Seq first
   float* score = nullptr;  // accumulation scratch: scores, then [B][nq] lse
   size_t score_cap = 0;
-  float* rec = nullptr;  // decode records, then tickets
-  size_t rec_cap = 0;    // floats
-  int* tickets = nullptr;
-  size_t tickets_cap = 0;
   int* status = nullptr;
   int sms = 0;
   bool has_empty = false;
@@ -160,11 +161,13 @@ int f8_resident(int d, int cluster, int dev) {
 // Few and short segments: a cluster per segment, merged in distributed
 // shared memory, when all the clusters are resident at once and a warp gets
 // at most kF8ClusterBlocks blocks.  One sequence of 4097 slots x 8 heads:
-// %CLUSTER% us, against %GLOBAL% us through records in global memory, whose
-// fence, ticket and loads take turns.
+// 10.2 us a call, against 15.6 us through records in global memory, whose
+// fence, ticket and loads take turns; 1089 slots x 4 heads of 256, 8.2 against
+// 15.3 us.  Above kF8ClusterBlocks the longer ranges cost more than the merge.
 // Else equal ranges of all items, or, where that leaves the longest range
 // within kF8Straddle blocks of it, ranges that end with the segments: a CTA
-// with parts of two segments merges twice.
+// with parts of two segments merges twice, 5 us in which the SM streams some
+// 50 blocks, half of which the SM's other CTA makes up for.
 int f8_partition(const molot_f8b_plan* p, const std::vector<F8Seq>& seqs,
                  const std::vector<int>& visit, int nkv, int HG, int d, std::vector<F8Cta>* out) {
   const int B = (int)seqs.size();
@@ -309,36 +312,26 @@ int f8_build(molot_f8b_plan* p, int B, int nq, int nkv, int d, const int* seq_le
     F8_CUDA(cudaMallocHost(&p->h_buf, total * sizeof(int)));
     p->h_cap = total;
   }
-  if (p->d_cap < total) {
-    F8_CUDA(cudaDeviceSynchronize());
-    cudaFree(p->d_buf);
-    p->d_buf = nullptr;
-    p->d_cap = 0;
-    const size_t cap = std::max<size_t>(total, 1024);
-    F8_CUDA(cudaMalloc(&p->d_buf, cap * sizeof(int)));
-    p->d_cap = cap;
-  }
   // decode scratch: two records a CTA, a ticket per segment
   const size_t rec = (size_t)2 * f8_ctas(d) * p->sms * (8 * (size_t)d + 16);
-  const size_t tickets = (size_t)B * nkv * ((nq / nkv + 7) / 8);
-  if (p->rec_cap < rec || p->tickets_cap < tickets) {
+  const size_t tickets = (size_t)B * nkv * HG;
+  if (p->d_cap < total || p->tickets_cap < tickets || p->rec_cap < rec) {
+    auto up = [](size_t n) { return (n + 63) / 64 * 64; };
+    const size_t nd = up(std::max<size_t>({total, p->d_cap, 4096}));
+    const size_t nt = up(std::max<size_t>({tickets, p->tickets_cap, 1024}));
+    const size_t nr = up(std::max(rec, p->rec_cap));
     F8_CUDA(cudaDeviceSynchronize());
-    if (p->rec_cap < rec) {
-      cudaFree(p->rec);
-      p->rec = nullptr;
-      p->rec_cap = 0;
-      F8_CUDA(cudaMalloc(&p->rec, rec * sizeof(float)));
-      p->rec_cap = rec;
-    }
-    if (p->tickets_cap < tickets) {
-      cudaFree(p->tickets);
-      p->tickets = nullptr;
-      p->tickets_cap = 0;
-      const size_t cap = std::max<size_t>(tickets, 1024);
-      F8_CUDA(cudaMalloc(&p->tickets, cap * sizeof(int)));
-      F8_CUDA(cudaMemsetAsync(p->tickets, 0, cap * sizeof(int), st));
-      p->tickets_cap = cap;
-    }
+    cudaFree(p->mem);
+    p->mem = nullptr;
+    p->d_cap = p->tickets_cap = p->rec_cap = 0;
+    F8_CUDA(cudaMalloc(&p->mem, (nd + nt + nr) * 4));
+    p->d_buf = reinterpret_cast<int*>(p->mem);
+    p->tickets = p->d_buf + nd;
+    p->rec = reinterpret_cast<float*>(p->tickets + nt);
+    F8_CUDA(cudaMemsetAsync(p->tickets, 0, nt * sizeof(int), st));
+    p->d_cap = nd;
+    p->tickets_cap = nt;
+    p->rec_cap = nr;
   }
   std::memcpy(p->h_buf, seqs.data(), B * sizeof(F8Seq));
   std::memcpy(p->h_buf + o_ctas, ctas.data(), grid * sizeof(F8Cta));
@@ -447,10 +440,8 @@ void molot_f8b_plan_destroy(molot_f8b_plan* p) {
   cudaSetDevice(p->device);
   cudaDeviceSynchronize();
   cudaFreeHost(p->h_buf);
-  cudaFree(p->d_buf);
+  cudaFree(p->mem);
   cudaFree(p->score);
-  cudaFree(p->rec);
-  cudaFree(p->tickets);
   cudaFree(p->status);
   cudaEventDestroy(p->uploaded);
   if (prev >= 0) cudaSetDevice(prev);
