@@ -63,7 +63,8 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 size_t act_bytes(int t) { return t == MOLOT_ACT_F32 ? 4 : 2; }
 
 constexpr int kF8ClusterBlocks = 12;  // blocks per warp up to which clusters merge
-constexpr int kF8Straddle = 24;       // blocks that a second merge is worth
+constexpr int kF8Straddle = 64;       // blocks that a second merge is worth
+constexpr int kF8Switch = 64;         // blocks (at d = 128) that a change of segments is worth
 
 // f(T{}, D) for an activation type and a head size.
 template <class F>
@@ -166,8 +167,9 @@ int f8_resident(int d, int cluster, int dev) {
 // 15.3 us.  Above kF8ClusterBlocks the longer ranges cost more than the merge.
 // Else equal ranges of all items, or, where that leaves the longest range
 // within kF8Straddle blocks of it, ranges that end with the segments: a CTA
-// with parts of two segments merges twice, 5 us in which the SM streams some
-// 50 blocks, half of which the SM's other CTA makes up for.
+// with parts of two segments merges twice, and that took it 12 us of the 44
+// in which the others streamed 223 blocks.  Where ranges do straddle, a
+// segment's change counts kF8Switch blocks.
 int f8_partition(const molot_f8b_plan* p, const std::vector<F8Seq>& seqs,
                  const std::vector<int>& visit, int nkv, int HG, int d, std::vector<F8Cta>* out) {
   const int B = (int)seqs.size();
@@ -223,8 +225,26 @@ int f8_partition(const molot_f8b_plan* p, const std::vector<F8Seq>& seqs,
   }
   const long long grid = std::min<long long>((items + kF8Warps - 1) / kF8Warps, max_grid);
   out->resize(grid);
-  auto start = [&](long long c) { return c * items / grid; };
-  auto owner = [&](long long x) { return ((x + 1) * grid + items - 1) / items - 1; };
+  // Equal ranges, a segment counting `extra` blocks more than it has: where
+  // CTA c's range starts.
+  const long long extra = std::min<long long>((long long)kF8Switch * 128 / d, items / grid / 4);
+  const long long cost = items + extra * segs;
+  std::vector<long long> starts(grid + 1, items);
+  {
+    long long v = 0, x = 0, c = 0;  // cost and items before the segment
+    for (int b = 0; b < B; ++b)
+      for (int seg = 0; seg < (seqs[b].nblk ? nkv * HG : 0); ++seg) {
+        const long long nb = seqs[b].nblk;
+        for (; c < grid && c * cost / grid < v + extra + nb; ++c)
+          starts[c] = x + std::max<long long>(0, c * cost / grid - v - extra);
+        v += extra + nb;
+        x += nb;
+      }
+  }
+  auto start = [&](long long c) { return starts[c]; };
+  auto owner = [&](long long x) {
+    return (long long)(std::upper_bound(starts.begin(), starts.begin() + grid, x) - starts.begin()) - 1;
+  };
   int b = 0;
   for (long long c = 0; c < grid; ++c) {
     F8Cta& k = (*out)[c];

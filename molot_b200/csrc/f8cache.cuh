@@ -236,18 +236,20 @@ struct F8Dec {
   static constexpr int LW = HB / 16;             // words of a K row's half per lane
   static constexpr int VB = D >= 128 ? 16 : 8;   // bytes of a V row's half per lane
   static constexpr int kCtas = D == 256 ? 1 : 2;
-  // Ring of blocks per warp: 192 KB an SM in flight
-  static constexpr int kStages = D == 64 ? 6 : 3;
+  // Ring of blocks per warp: 128 KB an SM in flight
+  static constexpr int kStages = D == 64 ? 4 : 2;
   static constexpr int kBlk = 2 * kF8Blk * D;  // bytes of K and V of a block
   static constexpr int kRing = kF8Warps * kStages * kBlk;
   static constexpr int kFrag = KS * 32 * 4;  // floats of O in fragment order
   static constexpr int kRec = kFrag + 16;    // + M[8], l[8]
   static constexpr int kQ = KS * 32 * 8;     // bytes of one FP16 part of Q
-  static constexpr int kBar = kRing + 2 * kQ + 64;
+  // the warps' records, or what a merge of 2 x 148 CTAs' records needs
+  static constexpr int kMerge = kF8Warps * kRec * 4 > 24 * 1024 ? kF8Warps * kRec * 4 : 24 * 1024;
+  static constexpr int kBar = kRing + kMerge + 2 * kQ + 64;
   // what a cluster's CTAs send here: 1 / C of each one's positions, M, l
   static constexpr int kPush = kBar + kF8Warps * kStages * 8;
   static constexpr int kSmem = kPush + kFrag * 4 + 16 * 64 + 1024;  // + alignment
-  static_assert(kRing >= kF8Warps * kRec * 4, "the warps' records take the ring's place");
+  static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "shared memory");
 };
 
 // TMA: box of 16 rows at byte x (0 or 128) and row y of a pool.
@@ -310,8 +312,8 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
   constexpr int kThreads = kF8Warps * 32;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
-  float* recs = reinterpret_cast<float*>(smem);  // [warps][kRec], after the ring
-  unsigned char* qs = smem + F::kRing;           // high part, then low
+  float* recs = reinterpret_cast<float*>(smem + F::kRing);  // [warps][kRec]
+  unsigned char* qs = smem + F::kRing + F::kMerge;          // high part, then low
   float* qinv = reinterpret_cast<float*>(qs + 2 * F::kQ);  // [8]
   __shared__ int s_last;
   __shared__ volatile int s_abort;
@@ -341,52 +343,66 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
   ptx::pdl_launch_dependents();
   __syncthreads();
 
+  // The warp's blocks of a piece (a segment's part) are i0 + warp + 8 m, m in
+  // [0, nm).  They are fetched kStages ahead, and a piece's first ones before
+  // the last one's merge; of a run of 32, lane l has block l's place and
+  // scales.  The f_ side is the piece that is being fetched.
+  int f_b = 0, f_h = 0, f_i0 = 0, f_nm = 0, place = 0, place_next = 0;
+  float ks_in = 0.f, vs_in = 0.f;
+  // block index within the pool; K and V of 180 GB hold fewer than 2^27
+  auto place_of = [&](int m) {
+    if (m >= f_nm) return 0;
+    const F8Seq& q = a.seqs[f_b];
+    const int i = f_i0 + warp + kF8Warps * m;
+    const int blk = i < q.na ? q.a0 + i : q.b0 + i - q.na;
+    const int page = a.pool.bt[(long long)f_b * a.pool.max_pages + blk / bpp];
+    return (int)(((long long)page * nkv + f_h) * bpp + blk % bpp);
+  };
+  auto fetch = [&](int m) {
+    if ((m & 31) == 0) {
+      if (m) place = place_next, place_next = place_of(m + 32 + lane);
+      if (m + lane < f_nm) {
+        ks_in = __ldg(a.pool.k_scale + place);
+        vs_in = __ldg(a.pool.v_scale + place);
+      }
+    }
+    if (lane == (m & 31)) {
+      const uint32_t dst = ring + st_put * F::kBlk;
+      ptx::mbar_arrive_expect_tx(full + st_put, F::kBlk);
+#pragma unroll
+      for (int i = 0; i < NH; ++i) {
+        tma_rows(dst + i * kF8Blk * 128, &mk, i * 128, place * kF8Blk, full + st_put);
+        tma_rows(dst + kF8Blk * D + i * kF8Blk * 128, &mv, i * 128, place * kF8Blk, full + st_put);
+      }
+    }
+    st_put = st_put + 1 == F::kStages ? 0 : st_put + 1;
+    ++asked;
+  };
+  auto begin = [&](int pb, int ph, int p0, int p1) {
+    f_b = pb, f_h = ph, f_i0 = p0;
+    f_nm = p1 - p0 > warp ? (p1 - p0 - warp + kF8Warps - 1) / kF8Warps : 0;
+    place = place_of(lane);
+    place_next = f_nm > 32 ? place_of(lane + 32) : 0;
+#pragma unroll 1
+    for (int m = 0; m < F::kStages; ++m)
+      if (m < f_nm) fetch(m);
+  };
+  int i1 = min(sq.nblk, i0 + left);
+  begin(b, seg / a.HG, i0, i1);
+
   // (a CTA of a cluster takes part in its merge even without blocks)
   for (bool go = left > 0 || a.cluster; go; go = left > 0) {
-    const int i1 = min(sq.nblk, i0 + left);
     const int h = seg / a.HG, hg = seg % a.HG;
     const int head0 = h * a.G + hg * 8, nh = min(8, a.G - hg * 8);
-    const int* bt = a.pool.bt + (long long)b * a.pool.max_pages;
-    const bool first_piece = left == cta.items;
+    const bool first_piece = left == cta.items, whole = !a.cluster && i0 == 0 && i1 == sq.nblk;
+    const int ob = b;  // the piece's sequence and heads, for its outputs
     left -= i1 - i0;
-
-    // The warp's blocks are i0 + warp + 8 m, m in [0, nm).  They are fetched
-    // kStages ahead; of a run of 32, lane l has block l's place and scales.
-    const int nm = i1 - i0 > warp ? (i1 - i0 - warp + kF8Warps - 1) / kF8Warps : 0;
+    const int nm = f_nm;
     auto block_of = [&](int m) {
       const int i = i0 + warp + kF8Warps * m;
       return i < sq.na ? sq.a0 + i : sq.b0 + i - sq.na;
     };
-    // block index within the pool; K and V of 180 GB hold fewer than 2^31
-    auto place_of = [&](int m) {
-      const int blk = m < nm ? block_of(m) : 0;
-      return m < nm ? (int)(((long long)bt[blk / bpp] * nkv + h) * bpp + blk % bpp) : 0;
-    };
-    int place = place_of(lane), place_next = nm > 32 ? place_of(lane + 32) : 0;
-    float ks_in = 0.f, vs_in = 0.f, ks_run = 0.f, vs_run = 0.f;
-    auto fetch = [&](int m) {
-      if ((m & 31) == 0) {
-        if (m) place = place_next, place_next = place_of(m + 32 + lane);
-        if (m + lane < nm) {
-          ks_in = __ldg(a.pool.k_scale + place);
-          vs_in = __ldg(a.pool.v_scale + place);
-        }
-      }
-      if (lane == (m & 31)) {
-        const uint32_t dst = ring + st_put * F::kBlk;
-        ptx::mbar_arrive_expect_tx(full + st_put, F::kBlk);
-#pragma unroll
-        for (int i = 0; i < NH; ++i) {
-          tma_rows(dst + i * kF8Blk * 128, &mk, i * 128, place * kF8Blk, full + st_put);
-          tma_rows(dst + kF8Blk * D + i * kF8Blk * 128, &mv, i * 128, place * kF8Blk, full + st_put);
-        }
-      }
-      st_put = st_put + 1 == F::kStages ? 0 : st_put + 1;
-      ++asked;
-    };
-#pragma unroll
-    for (int m = 0; m < F::kStages; ++m)
-      if (m < nm) fetch(m);
+    float ks_run = 0.f, vs_run = 0.f;
 
     // Q in operand order, a warp per head
     {
@@ -587,13 +603,24 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
       if (m + F::kStages < nm) fetch(m + F::kStages);
     }
 
+    // the next segment, of the next sequence that sees anything, on its way
+    if (left > 0) {
+      i0 = 0;
+      if (++seg == nkv * a.HG) {
+        seg = 0;
+        do sq = a.seqs[++b];
+        while (sq.nblk == 0);
+      }
+      i1 = min(sq.nblk, left);
+      begin(b, seg / a.HG, i0, i1);
+    }
+
     // merge the warps: records in fragment order, then one sum per position
 #pragma unroll
     for (int k = 4; k < 32; k <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, k);
       l1 += __shfl_xor_sync(0xffffffffu, l1, k);
     }
-    __syncthreads();  // every warp is done with the ring
     {
       float* r = recs + warp * F::kRec;
 #pragma unroll
@@ -622,7 +649,7 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
         if (hh + y >= nh) continue;
         const float l = y ? ll.y : ll.x;
         const float inv = l > 0.f || l != l ? 0x1p32f / l : 0.f;
-        const long long row = (long long)b * a.nq + head0 + hh + y;
+        const long long row = (long long)ob * a.nq + head0 + hh + y;
         T* op = static_cast<T*>(a.o) + row * D + dim;
         Act<T>::store(op, (y ? acc.y : acc.x) * inv);
         Act<T>::store(op + 1, (y ? acc.w : acc.z) * inv);
@@ -633,7 +660,6 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
         }
       }
     };
-    const bool whole = !a.cluster && i0 == 0 && i1 == sq.nblk;
     float* rec = a.rec + (2 * (long long)blockIdx.x + (first_piece ? 0 : 1)) * F::kRec;
     // a cluster's CTA r merges positions [r * per, (r + 1) * per)
     const int C = a.cluster, per = C ? np / C : 0;
@@ -710,7 +736,7 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
       __threadfence();
       __syncthreads();
       if (tid == 0) {
-        int* tk = a.tickets + ((long long)b * nkv + h) * a.HG + hg;
+        int* tk = a.tickets + ((long long)ob * nkv + h) * a.HG + hg;
         const bool last = ptx::atom_add_acq_rel_gpu(tk, 1) == n - 1;
         if (last) *tk = 0;
         s_last = last;
@@ -723,7 +749,7 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
           return a.rec + (long long)(k ? (rec0 & ~1) + 2 * k : rec0) * F::kRec;
         };
         // factors of the records: [n][8] M, then l, then the heads' M, l
-        float* fac = reinterpret_cast<float*>(smem);
+        float* fac = recs;
         float* fl = fac + n * 8;
         float* tot = fl + n * 8;  // M[8], l[8]
         for (int i = tid; i < n * 8; i += kThreads) {
@@ -782,17 +808,7 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
         }
       }
     }
-    // shared memory is free for the next segment's copies
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();
-    if (left > 0) {  // the next segment, of the next sequence that sees anything
-      i0 = 0;
-      if (++seg == nkv * a.HG) {
-        seg = 0;
-        do sq = a.seqs[++b];
-        while (sq.nblk == 0);
-      }
-    }
+    __syncthreads();  // records and Q are free for the next piece
   }
   if (s_abort)  // copies in flight end before the CTA does
     for (int k = max(0, asked - F::kStages); k < asked; ++k)
