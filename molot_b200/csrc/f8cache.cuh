@@ -104,8 +104,9 @@ struct F8WriteArgs {
 };
 
 // A warp per touched block, head and pool: the new rows' magnitude, the
-// block's scale, the codes.  Bound by bytes.  The older rows of a partly
-// filled block are read only when its scale grows.
+// block's scale, the codes.  Bound by bytes: 24760 FP32 rows of 8 heads of 128
+// took 47.5 us, 5.3 TB/s; 64 rows of a decode step take a launch, 3.4 us.
+// The older rows of a partly filled block are read only when its scale grows.
 template <class T, int D>
 __global__ void __launch_bounds__(128) f8_write_kernel(const __grid_constant__ F8WriteArgs a) {
   constexpr int EPL = Act<T>::EPL, NC = kF8Blk * D / EPL / 32;
@@ -176,11 +177,12 @@ __global__ void __launch_bounds__(128) f8_write_kernel(const __grid_constant__ F
 // Work.  An item is one 16-slot block of one kv head for up to 8 of its
 // query heads (a head group; nq / nkv above 8 makes several).  Items are
 // numbered sequence by sequence, segment by segment (sequence, kv head, head
-// group) and block by block, and every CTA takes an equal contiguous range,
-// whatever the raggedness.  A warp takes one block at a time.  A segment
-// inside one CTA is finished there; one that several share leaves a record
-// per CTA (reference, sum, unnormalised output), merged by the last CTA to
-// finish, in CTA order.
+// group) and block by block; a CTA takes a range of them that the plan chose
+// (f8_partition), a warp one block at a time.  A segment inside one CTA is
+// finished there.  One that several CTAs share is merged by its cluster in
+// distributed shared memory (short launches), or from a record per CTA
+// (reference, sum, unnormalised output) by the last of them to finish, in CTA
+// order whoever that is.
 //
 // Mathematics.  The products run on the tensor cores with the slots in the
 // rows: S^T [16 slots x 8 heads] = K Q^T and O^T [d x 8 heads] += V^T P^T by
@@ -200,9 +202,14 @@ __global__ void __launch_bounds__(128) f8_write_kernel(const __grid_constant__ F
 // <= 2^14 multiplies the codes, while l adds 2^(s - M + 38), which stays
 // within FP32 for every ev in [-64, 120].  O = sum(P * code) * 2^32 / l.
 //
-// Bound by the bytes of the cache, so by what is in flight: with one block
-// of a warp under way in registers (64 KB an SM) the 2.35 M slots x 8 heads
-// of d = 128 took 993 us, nothing else above 45 % busy.
+// Bound by the bytes of the cache, and by the latency of a warp's chain from
+// a block's arrival to its weights: 2.35 M slots x 8 heads of 128 (4.29 GB,
+// FP32 queries in groups of 8) took 816 us, 5.3 TB/s; 1.02 M slots (2.16 GB,
+// BF16, groups of 4) 385 us, 5.4 TB/s, the tensor pipe 28 and 16 % busy, no
+// pipe above 40 %.  Steps on the way (the first case): operands straight from
+// 16-byte global loads 1030 us, staged by cp.async 1257, by TMA 886; then the
+// ranges, the next segment's blocks asked for before a merge, and less
+// arithmetic per block.
 struct F8DecodeArgs {
   F8Pool pool;
   const F8Seq* seqs;
@@ -840,8 +847,9 @@ constexpr int kF8WeightSlots = 4;  // slots per thread of the counter kernel
 
 // Counters: wout = win + the slot's weights summed over the kv head's group,
 // from the scores that the decode left.  Heads are summed in order, so the
-// sum does not depend on the launch.  Bound by the scores' bytes; each thread
-// has its slots' loads in flight together.
+// sum does not depend on the launch.  Bound by the scores' bytes (1.02 M slots
+// x 32 heads: 130 MB written by the decode and read here, some 50 us of the
+// two launches' 427); each thread has its slots' loads in flight together.
 __global__ void __launch_bounds__(128) f8_weight_kernel(const __grid_constant__ F8WeightArgs a) {
   const int g = blockIdx.y, b = blockIdx.z;
   const F8Seq sq = a.seqs[b];
@@ -927,9 +935,10 @@ constexpr int kF8SelKeys = 48 * 1024;
 // The slots to keep of one sequence and kv head, ascending: a radix select
 // of the (budget - recent)-th largest key over slots [0, n - recent), 8 bits
 // a pass until a bucket is taken whole, then an ordered compaction: keys above the threshold, and the
-// lowest slots among those equal to it.  One sequence of 4351 slots x 8
-// heads, and 16 of up to 32768, took 37 and 95 us with the keys read from
-// the pool in each pass and one thread walking the histogram.
+// lowest slots among those equal to it.  Bound by latency, the passes taking
+// turns in one CTA: 16 sequences of up to 32768 slots x 8 heads take 32 us (94
+// with the keys read from the pool in each pass and one thread walking the
+// histogram).
 __global__ void __launch_bounds__(kF8SelThreads) f8_select_kernel(const __grid_constant__ F8EvictArgs a) {
   extern __shared__ uint32_t keys[];
   const int g = blockIdx.x, b = blockIdx.y;
@@ -1111,8 +1120,8 @@ __device__ __forceinline__ uint32_t f8_rescale4(uint32_t c, __half2 f) {
 // A warp per destination block and head: 16 kept rows of K and of V from
 // anywhere in the sequence, their common scales, their codes.  Bound by
 // bytes; the arithmetic stays on packed codes (magnitudes compared as bytes,
-// rows whose scale changes multiplied in FP16 pairs): on FP32 values it
-// took 82 us where the bytes of 16 x 4096 slots x 8 heads take 41.
+// rows whose scale changes multiplied in FP16 pairs): 16 x 4096 slots x 8
+// heads, 268 MB, take 60 us, 4.5 TB/s; on FP32 values they took 82.
 template <int D>
 __global__ void __launch_bounds__(128) f8_move_kernel(const __grid_constant__ F8EvictArgs a) {
   constexpr int NC = kF8Blk * D / 16 / 32;  // 16-byte chunks per lane
