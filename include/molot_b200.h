@@ -59,8 +59,8 @@ int molot_device_status(int clear);
  * copy in flight, the launch records MOLOT_ERR_TIMEOUT in the status word of
  * the workspace it used and its outputs are garbage.  Nothing faults, traps
  * or hangs.  wait_limit_ns = 0 cancels a pending request.  For tests of the
- * status path (molot_kv_check, molot_paged_check, molot_device_status,
- * molot_noalloc_status); never set in production. */
+ * status path (molot_kv_check, molot_paged_check, molot_f8b_check,
+ * molot_device_status, molot_noalloc_status); never set in production. */
 int molot_debug_withhold_next(unsigned long long wait_limit_ns);
 
 /* ------------------------------------------------------------------------

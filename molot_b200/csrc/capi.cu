@@ -604,6 +604,13 @@ int max_active_clusters(const KernelRef& k, int cluster, int dev) {
 // molot_debug_withhold_next: pending request of the calling host thread.
 thread_local unsigned long long g_withhold_ns = 0;
 
+// The request, for a launch of another translation unit (0: none).
+unsigned long long take_withhold_ns() {
+  const unsigned long long ns = g_withhold_ns;
+  g_withhold_ns = 0;
+  return ns;
+}
+
 void take_withhold(DecodeArgs& a) {
   if (!g_withhold_ns) return;
   a.withhold = 1;

@@ -18,6 +18,7 @@
 
 namespace molot {
 int set_last_error(int code, const char* msg);
+unsigned long long take_withhold_ns();  // molot_debug_withhold_next
 
 namespace {
 
@@ -560,7 +561,9 @@ int molot_f8b_decode(molot_f8b_plan* p, const molot_f8b_layer* layer, const void
   a.cluster = p->cluster;
   a.has_empty = p->has_empty;
   a.status = p->status;
-  a.timeout_ns = kF8WaitNs;
+  const unsigned long long withheld = take_withhold_ns();
+  a.withhold = withheld != 0;
+  a.timeout_ns = withheld ? withheld : kF8WaitNs;
   a.scale = scale;
   a.cap = softcap;
   CUtensorMap mk, mv;

@@ -227,6 +227,7 @@ struct F8DecodeArgs {
   int B, nq, G, HG;  // HG head groups of up to 8 per kv head
   int cluster;       // CTAs of a cluster, a segment each; 0: records in global memory
   int has_empty;     // some sequence sees nothing
+  int withhold;      // test hook: no copies, so that the first wait runs out
   int* status;       // 1 after a bounded wait ran out
   unsigned long long timeout_ns;
   float scale, cap;
@@ -373,7 +374,7 @@ __global__ void __launch_bounds__(kF8Warps * 32, F8Dec<T, D>::kCtas)
         vs_in = __ldg(a.pool.v_scale + place);
       }
     }
-    if (lane == (m & 31)) {
+    if (lane == (m & 31) && !a.withhold) {
       const uint32_t dst = ring + st_put * F::kBlk;
       ptx::mbar_arrive_expect_tx(full + st_put, F::kBlk);
 #pragma unroll

@@ -12,8 +12,8 @@
 //
 // Per key tile j and row tile s:  S_s = Q_s K_j^T (tcgen05.mma, both operands
 // in shared memory, brought by TMA with the 128-byte swizzle);  the row
-// tile's warpgroup reads its rows of S (a thread per row, so maxima and sums
-// never leave the thread), applies cap, bias and mask, and writes
+// tile's threads read their rows of S (a thread per row, so maxima and sums
+// never leave the thread; at d = 256 two, half of the keys each), apply cap, bias and mask, and write
 // P = 2^(x - m) in the operands' type over S's columns, in two halves;
 // O_s += P V_j with P from tensor memory and V as an MN-major operand,
 // straight as TMA brought it.  m is raised, and O rescaled, only when a score
@@ -33,7 +33,8 @@
 // zeros in the place of infinities and NaN, and name the keys; a row that
 // does see such a key becomes NaN.
 //
-// Warps: 0-3 (4-7) softmax of row tile 0 (1), epilogue; then one that issues
+// Warps: 0-3 (4-7) softmax of row tile 0 (1), or of the first (second) half of
+// the keys at d = 256, epilogue; then one that issues
 // TMA copies, one that issues MMAs, two idle, four that look over V.  Every
 // wait is bounded; one that runs out records a status code and ends the CTA.
 //
@@ -44,8 +45,9 @@
 // chain is 110 reading S, 550 to the maximum, 1500 exponentials (1024 of the
 // MUFU), 230 storing P, 1050 for PV and QK.  Not kept: part of the
 // exponentials as polynomials on the FMA pipe (1.5 % faster alone, 1 % slower
-// back to back); two threads a row (the registers that a thread then has
-// spill); one row tile and two CTAs an SM (5 % slower: K and V come twice).
+// back to back); two threads a row at d <= 128 (the registers that a
+// thread then has spill; at d = 256 they took 8192 windowed rows from 143 to
+// 131 us, tiles of 128 keys, K and V without a second buffer, 156); one row tile and two CTAs an SM (5 % slower: K and V come twice).
 #pragma once
 
 #include <cuda.h>
@@ -81,6 +83,7 @@ struct PackedArgs {
 template <int D>
 struct PackedShape {
   static constexpr int kTiles = D == 256 ? 1 : 2;   // row tiles of a CTA
+  static constexpr int kHalves = 2 / kTiles;        // threads of a row, half of the keys each
   static constexpr int BN = D == 256 ? 64 : 128;    // keys of a tile
   static constexpr int kBufs = 2;                   // S buffers in all
   // K / V ring, K and V in turn; at d = 64 long enough that no second CTA,
@@ -90,9 +93,10 @@ struct PackedShape {
   static constexpr int kQ = 128 * D * 2;            // bytes of a Q tile
   static constexpr int kKV = BN * D * 2;            // bytes of a ring slot
   static constexpr int kBar = kTiles * kQ + kSlots * kKV;
-  static constexpr int kSmem = kBar + 512 + 1024;   // + alignment
+  static constexpr int kXch = kBar + 512;           // what a row's halves exchange
+  static constexpr int kSmem = kXch + 2048 + 1024;  // + alignment
   static constexpr uint32_t kS = 0, kO = kBufs * BN;  // tensor-memory columns
-  static constexpr int kSoft = 128 * kTiles;        // softmax threads
+  static constexpr int kSoft = 256;                 // softmax threads
   static constexpr int kThreads = kSoft + 256;
   static_assert(kO + kTiles * D <= 512, "tensor memory");
   static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -177,11 +181,10 @@ __device__ __forceinline__ void st32(uint32_t addr, const uint32_t* r) {
       PK_R8(r, 0), PK_R8(r, 8), PK_R8(r, 16), PK_R8(r, 24)
       : "memory");
 }
-__device__ __forceinline__ void st16(uint32_t addr, const uint32_t* r) {
+__device__ __forceinline__ void st8(uint32_t addr, const uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-      "%14,%15,%16};" ::"r"(addr),
-      PK_R8(r, 0), PK_R8(r, 8)
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr),
+      PK_R8(r, 0)
       : "memory");
 }
 __device__ __forceinline__ void wait_st() {
@@ -230,7 +233,8 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
     packed_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                   const __grid_constant__ CUtensorMap mv, const __grid_constant__ PackedArgs a) {
   using S = PackedShape<D>;
-  constexpr int BN = S::BN, NT = S::kTiles;
+  constexpr int BN = S::BN, NT = S::kTiles, HV = S::kHalves;
+  constexpr int HN = BN / HV;  // keys of a softmax thread
   constexpr bool kBf = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
@@ -282,8 +286,8 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(s_full + i, 1);
-      ptx::mbar_init(p_full + i, 128);
-      ptx::mbar_init(p_half + i, 128);
+      ptx::mbar_init(p_full + i, 128 * HV);
+      ptx::mbar_init(p_half + i, 128 * HV);
     }
     ptx::mbar_init(o_full, 1);
     ptx::mbar_init(q_full, 1);
@@ -318,11 +322,12 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
   if (warp < kTmaWarp) {
     // ------------------------------------------------------------- softmax
     // 512 threads x 128 registers: 256 x 200 + 256 x 56
-    if constexpr (NT == 2) ptx::setmaxnreg_inc<200>();
-    const int tile = warp >> 2;
-    const int r = tid & 127;
+    ptx::setmaxnreg_inc<200>();
+    const int tile = NT == 2 ? warp >> 2 : 0, half = HV == 2 ? warp >> 2 : 0;
+    const int r = tid & 127, k0 = half * HN;
+    float* xch = reinterpret_cast<float*>(smem + S::kXch);  // [2][half][row]
     const uint32_t lane_base = tm + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t o_col = lane_base + S::kO + tile * D;
+    const uint32_t o_col = lane_base + S::kO + tile * D + half * (D / HV);
     const int pl = r / a.G, hd = r - pl * a.G;
     const int m = it.m0 + tile * a.BP + pl;
     const bool valid = pl < a.BP && m < it.m_rows;
@@ -354,20 +359,20 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
       wait(s_full + buf, (NT == 2 ? j : j >> 1) & 1, 1);
       __syncwarp();
       pk::fence_after();
-      uint32_t s[BN];
+      uint32_t s[HN];
 #pragma unroll
-      for (int c = 0; c < BN; c += 32) pk::ld32(s_col + c, s + c);
+      for (int c = 0; c < HN; c += 32) pk::ld32(s_col + k0 + c, s + c);
 #pragma unroll
-      for (int c = 0; c < BN; c += 32) pk::wait_ld(s + c);
+      for (int c = 0; c < HN; c += 32) pk::wait_ld(s + c);
       const int t0 = tile_of(j) * BN;
       const bool edge = !whole(t0);
       if (kMode == kCap) {
         float am = 0.f;
 #pragma unroll
-        for (int i = 0; i < BN; ++i) am = fmaxf(am, fabsf(__uint_as_float(s[i])));
+        for (int i = 0; i < HN; ++i) am = fmaxf(am, fabsf(__uint_as_float(s[i])));
         if (__any_sync(0xffffffffu, !(am * fabsf(in) <= kCapPoly))) {
 #pragma unroll
-          for (int i = 0; i < BN; ++i) {
+          for (int i = 0; i < HN; ++i) {
             const float x = __uint_as_float(s[i]), y = x * in, y2 = y * y;
             float q = ct[5];
 #pragma unroll
@@ -377,7 +382,7 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < BN; i += 2) {
+          for (int i = 0; i < HN; i += 2) {
             const float2 x = make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
             const float2 y = __fmul2_rn(x, make_float2(in, in)), y2 = __fmul2_rn(y, y);
             float2 q = make_float2(ct[5], ct[5]);
@@ -389,14 +394,14 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
         }
       }
       if (kMode == kBias || (kMode == kCap && a.slopes)) {
-        const float mul = kMode == kBias ? sl : 1.f, d0 = (float)(t0 - pos);
+        const float mul = kMode == kBias ? sl : 1.f, d0 = (float)(t0 + k0 - pos);
         if (it.prefix == 0 || t0 + BN - 1 <= pos0) {
           // no row sees keys beyond itself: -slope |pos - t| = slope (t - pos)
           float2 off[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) off[k] = make_float2(slope * (2 * k), slope * (2 * k + 1));
 #pragma unroll
-          for (int i = 0; i < BN; i += 8) {
+          for (int i = 0; i < HN; i += 8) {
             const float base = slope * (d0 + (float)i);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -409,7 +414,7 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < BN; ++i)
+          for (int i = 0; i < HN; ++i)
             s[i] = __float_as_uint(
                 fmaf(__uint_as_float(s[i]), mul, -slope * fabsf(d0 + (float)i)));
         }
@@ -419,25 +424,33 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
         const int slot = j % S::kVSlots;
         wait(kv_ok + slot, (j / S::kVSlots) & 1, 2);
 #pragma unroll
-        for (int c = 0; c < BN; c += 32) {
-          const uint32_t see =
-              pk::bits(r_lo - t0 - c, r_hi - t0 - c) | pk::bits(0, r_pre - t0 - c);
+        for (int c = 0; c < HN; c += 32) {
+          const int t = t0 + k0 + c;
+          const uint32_t see = pk::bits(r_lo - t, r_hi - t) | pk::bits(0, r_pre - t);
           if (!__all_sync(0xffffffffu, see == 0xffffffffu)) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (!((see >> i) & 1)) s[c + i] = 0xff800000u;
           }
-          if (bad[slot * 4 + c / 32] & see) l = CUDART_NAN_F;
+          if (bad[slot * 4 + (k0 + c) / 32] & see) l = CUDART_NAN_F;
         }
       }
       float mc4[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-      for (int i = 0; i < BN; i += 8)
+      for (int i = 0; i < HN; i += 8)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           mc4[k] = fmaxf(fmaxf(mc4[k], __uint_as_float(s[i + 2 * k])),
                          __uint_as_float(s[i + 2 * k + 1]));
-      const float mc = fmaxf(fmaxf(mc4[0], mc4[1]), fmaxf(mc4[2], mc4[3]));
+      float mc = fmaxf(fmaxf(mc4[0], mc4[1]), fmaxf(mc4[2], mc4[3]));
+      if constexpr (HV == 2) {
+        // the row's other half; the barrier also says that all of S is read,
+        // over which P goes
+        float* ex = xch + (j & 1) * 256;
+        ex[tid] = mc;
+        ptx::named_bar_sync(1, 256);
+        mc = fmaxf(mc, ex[tid ^ 128]);
+      }
       const bool raise = (mc - mx) * unit > 8.f || (mx == -CUDART_INF_F && mc > mx);
       if (__any_sync(0xffffffffu, raise)) {
         const bool resc = raise && mx != -CUDART_INF_F;
@@ -451,7 +464,7 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
             pk::fence_after();
           }
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
+          for (int c = 0; c < D / HV; c += 32) {
             uint32_t o[32];
             pk::ld32(o_col + c, o);
             pk::wait_ld(o);
@@ -466,10 +479,10 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
       const float neg = mx == -CUDART_INF_F ? 0.f : -mx;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < BN; c += BN / 2) {
-        uint32_t p[BN / 4];
+      for (int c = 0; c < HN; c += HN / 2) {
+        uint32_t p[HN / 4];
 #pragma unroll
-        for (int i = 0; i < BN / 4; ++i) {
+        for (int i = 0; i < HN / 4; ++i) {
           float2 z = __fadd2_rn(make_float2(__uint_as_float(s[c + 2 * i]),
                                             __uint_as_float(s[c + 2 * i + 1])),
                                 make_float2(neg, neg));
@@ -478,10 +491,11 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
           sum[i & 1] = __fadd2_rn(sum[i & 1], z);
           p[i] = pk::pack2<T>(z.x, z.y);
         }
-        if (BN == 128)
-          pk::st32(s_col + c / 2, p);
+        const uint32_t col = s_col + (k0 + c) / 2;
+        if constexpr (HN == 128)
+          pk::st32(col, p);
         else
-          pk::st16(s_col + c / 2, p);
+          pk::st8(col, p);
         pk::wait_st();
         pk::fence_before();
         ptx::mbar_arrive((c ? p_full : p_half) + buf);
@@ -489,6 +503,12 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
       l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
     }
     // epilogue
+    if constexpr (HV == 2) {  // the row's sum over both halves
+      ptx::named_bar_sync(1, 256);  // the last exchange has been read
+      xch[tid] = l;
+      ptx::named_bar_sync(1, 256);
+      l += xch[tid ^ 128];
+    }
     if (ntiles > 0) {
       wait(o_full, 0, 3);
       __syncwarp();
@@ -502,7 +522,7 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
     constexpr int kPieces = D / 8;  // of a row
     // (compact loops: code that runs once per CTA is fetched cold)
 #pragma unroll 1
-    for (int c = 0; c < D; c += 32) {
+    for (int c = 0; c < D / HV; c += 32) {
       uint32_t o[32];
       if (ntiles > 0) {
         pk::ld32(o_col + c, o);
@@ -516,26 +536,29 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
           w[k] = ntiles > 0 ? pk::pack2<T>(__uint_as_float(o[i + 2 * k]) * inv,
                                            __uint_as_float(o[i + 2 * k + 1]) * inv)
                             : 0u;
-        *reinterpret_cast<uint4*>(rows + lane * (D * 2) + (((c + i) / 8 ^ (lane & 7)) * 16)) =
+        *reinterpret_cast<uint4*>(rows + lane * (D * 2) + (((half * (D / HV) + c + i) / 8 ^ (lane & 7)) * 16)) =
             make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    __syncwarp();
+    if constexpr (HV == 2)
+      ptx::named_bar_sync(1, 256);  // the warps of both halves fill the same rows, and store half each
+    else
+      __syncwarp();
     // where the warp's rows go (-1: nowhere), a lane each
     const long long dst = valid ? row : -1;
 #pragma unroll 4
-    for (int k = 0; k < kPieces; ++k) {
-      const int i = lane + 32 * k, rr = i / kPieces, piece = i % kPieces;
+    for (int k = 0; k < kPieces / HV; ++k) {
+      const int i = lane + 32 * (k + half * (kPieces / HV)), rr = i / kPieces, piece = i % kPieces;
       const long long to = __shfl_sync(0xffffffffu, dst, rr);
       const uint4 v =
           *reinterpret_cast<const uint4*>(rows + rr * (D * 2) + ((piece ^ (rr & 7)) * 16));
       if (to >= 0) reinterpret_cast<uint4*>(static_cast<T*>(a.o) + to * D)[piece] = v;
     }
-    if (valid && a.lse)
+    if (valid && a.lse && half == 0)
       a.lse[row] = l == 0.f ? -CUDART_INF_F : (mx * unit + log2f(l)) * kLn2;
     pk::fence_before();
   } else {
-    if constexpr (NT == 2) ptx::setmaxnreg_dec<56>();
+    ptx::setmaxnreg_dec<56>();
     if (warp == kTmaWarp) {
       // ---------------------------------------------------------- copies
       if (lane == 0 && ntiles > 0) {
@@ -578,7 +601,9 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
           const uint64_t v = dv + (uint32_t)(slot * (S::kKV >> 4));
 #pragma unroll
           for (int c = 0; c < BN / 32; ++c) {
-            const int x = half * (BN / 32) + c;
+            // half of every softmax thread's keys
+            constexpr int kN = HN / 32;  // steps of 16 keys in it
+            const int x = c / kN * 2 * kN + half * kN + c % kN;
             pk::mma_ts(S::kO + tile * D, S::kS + buf * BN + x * 8, v + (x * 2048 >> 4),
                        id_o, !first || x > 0, go);
           }
@@ -599,6 +624,7 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
           if (NT == 1 && next) {  // the other S buffer
             pk::fence_after();
             qk(0, (j + 1) & 1, ks);
+            pk::commit(empty + ks, go);
           }
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
@@ -615,7 +641,7 @@ __global__ void __launch_bounds__(PackedShape<D>::kThreads, 1)
           if (!ok) break;
           if (NT == 1) pk::commit(pv_done, go);
           pk::commit(empty + vs, go);
-          if (next) pk::commit(empty + ks, go);
+          if (NT == 2 && next) pk::commit(empty + ks, go);
           vs += 2;
           if (vs >= S::kSlots) vs -= S::kSlots, vp ^= 1;
         }

@@ -155,3 +155,31 @@ def test_evict_many(mb, torch_cuda, n, budget, recent):
         want = torch.cat([order.sort()[0], t[n - recent:]])
         assert torch.equal(kept[0, h].long(), want)
         assert torch.equal(w[bt2[0].long()[j // ps], h, j % ps], c[want])
+
+
+def test_bounded_wait_is_reported(mb, torch_cuda):
+    """A decode whose copies are withheld gives up, reports it once, and
+    leaves the plan usable (nothing is in flight, nothing faults)."""
+    torch = torch_cuda
+    g = torch.Generator(device="cuda")
+    g.manual_seed(9)
+    n, nkv, d, ps = 300, 2, 64, 16
+    k, v, ks, vs = pools(torch, 19, nkv, ps, d, g)
+    bt = torch.arange(19, dtype=torch.int32, device="cuda").view(1, -1)
+    layer = mb.F8Layer(k, v, ks, vs, bt)
+    q = torch.randn(1, 4, d, device="cuda", generator=g)
+    o, o2 = torch.empty_like(q), torch.empty_like(q)
+    plan = mb.F8Plan()
+    plan.build(4, nkv, d, [n])
+    plan.decode(layer, q, o, 0.125)
+    plan.check()
+    mb.debug_withhold_next(1_000_000)
+    plan.decode(layer, q, o2, 0.125)
+    with pytest.raises(mb.MolotError) as e:
+        plan.check()
+    assert e.value.status == mb.ERR_TIMEOUT
+    plan.check()
+    plan.decode(layer, q, o2, 0.125)
+    plan.check()
+    assert torch.equal(o, o2)
+    plan.close()
