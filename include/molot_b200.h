@@ -2,7 +2,7 @@
  *
  * Drop-in replacement for the decode-attention path of Molot
  * (include/molot/attn.h and its call site in include/molot/forward.h).  All
- * arithmetic is FP32.  Every entry point returns an int status (MOLOT_OK or
+ * arithmetic is FP32 unless an entry says otherwise.  Every entry point returns an int status (MOLOT_OK or
  * a negative MOLOT_ERR_*) and never throws across the ABI.
  *
  * Conventions

@@ -61,6 +61,7 @@ int pk_bn(int d) { return d == 256 ? PackedShape<256>::BN : PackedShape<128>::BN
 int pk_build(molot_packed_plan* p, int ndocs, const int* q_lens, const int* k_lens,
              const int* prefix, int window, int nq, int nkv, int d, cudaStream_t st) {
   std::vector<std::pair<int, PackedItem>> items;  // with their key tiles
+  if (window >= 1 << 30) window = 0;              // no document is longer
   const int bp = 128 / (nq / nkv), step = bp * pk_tiles(d), bn = pk_bn(d);
   long long q0 = 0, k0 = 0;
   for (int i = 0; i < ndocs; ++i) {

@@ -66,6 +66,7 @@ CASES = {
     "prefix_negative": dict(q=[100], k=[30], nq=2, nkv=1, d=64, prefix=[12]),
     "bias_cap_all": dict(q=[400, 129], k=[700, 129], nq=8, nkv=2, d=128, prefix=[150, 7],
                          window=200, cap=10.0, bias=True),
+    "window_unlimited": dict(q=[100, 40], k=[30, 200], nq=4, nkv=2, d=64, window=2 ** 31 - 1),
     "group1": dict(q=[190], nq=3, nkv=3, d=128),
     "group8": dict(q=[190, 33], nq=16, nkv=2, d=128, bias=True),
     "group5": dict(q=[140], nq=5, nkv=1, d=64),
