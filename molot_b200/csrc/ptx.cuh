@@ -89,6 +89,12 @@ __device__ __forceinline__ uint64_t policy_evict_first() {
   return pol;
 }
 
+__device__ __forceinline__ uint64_t policy_evict_normal() {
+  uint64_t pol;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(pol));
+  return pol;
+}
+
 // One-dimensional TMA bulk copy global -> this CTA's shared memory; completion
 // is reported as `bytes` transactions on `bar`.  dst, src and bytes must be
 // multiples of 16.
