@@ -204,12 +204,12 @@ __global__ void __launch_bounds__(128) f8_write_kernel(const __grid_constant__ F
 //
 // Bound by the bytes of the cache, and by the latency of a warp's chain from
 // a block's arrival to its weights: 2.35 M slots x 8 heads of 128 (4.29 GB,
-// FP32 queries in groups of 8) took 816 us, 5.3 TB/s; 1.02 M slots (2.16 GB,
-// BF16, groups of 4) 385 us, 5.4 TB/s, the tensor pipe 28 and 16 % busy, no
-// pipe above 40 %.  Steps on the way (the first case): operands straight from
+// FP32 queries in groups of 8) take 816 to 874 us, 4.9 to 5.3 TB/s; 1.02 M
+// slots (2.16 GB, BF16, groups of 4) 380 us, 5.6 TB/s, the tensor pipe 28 and
+// 16 % busy, no pipe above 40 %.  Steps on the way (the first case): operands straight from
 // 16-byte global loads 1030 us, staged by cp.async 1257, by TMA 886; then the
-// ranges, the next segment's blocks asked for before a merge, and less
-// arithmetic per block.
+// ranges, the next segment's blocks asked for before a merge, less arithmetic
+// per block, and the L2 policy.
 struct F8DecodeArgs {
   F8Pool pool;
   const F8Seq* seqs;
@@ -856,7 +856,7 @@ constexpr int kF8WeightSlots = 4;  // slots per thread of the counter kernel
 // from the scores that the decode left.  Heads are summed in order, so the
 // sum does not depend on the launch.  Bound by the scores' bytes (1.02 M slots
 // x 32 heads: 130 MB written by the decode and read here, some 50 us of the
-// two launches' 427); each thread has its slots' loads in flight together.
+// two launches' 430); each thread has its slots' loads in flight together.
 __global__ void __launch_bounds__(128) f8_weight_kernel(const __grid_constant__ F8WeightArgs a) {
   const int g = blockIdx.y, b = blockIdx.z;
   const F8Seq sq = a.seqs[b];
