@@ -206,10 +206,10 @@ __global__ void __launch_bounds__(128) f8_write_kernel(const __grid_constant__ F
 // a block's arrival to its weights: 2.35 M slots x 8 heads of 128 (4.29 GB,
 // FP32 queries in groups of 8) take 816 to 874 us, 4.9 to 5.3 TB/s; 1.02 M
 // slots (2.16 GB, BF16, groups of 4) 380 us, 5.6 TB/s, the tensor pipe 28 and
-// 16 % busy, no pipe above 40 %.  Steps on the way (the first case): operands straight from
-// 16-byte global loads 1030 us, staged by cp.async 1257, by TMA 886; then the
-// ranges, the next segment's blocks asked for before a merge, less arithmetic
-// per block, and the L2 policy.
+// 16 % busy, no pipe above 40 %.  Steps on the way (the first case): operands
+// straight from 16-byte global loads 1030 us, staged by cp.async 1257, by TMA
+// 886; then the ranges, the next segment's blocks asked for before a merge,
+// less arithmetic per block, and the L2 policy.
 struct F8DecodeArgs {
   F8Pool pool;
   const F8Seq* seqs;
